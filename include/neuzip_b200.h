@@ -42,6 +42,7 @@ extern "C" {
 #define NZ_STATUS_BAD_STATE 0x8u   /* a lane did not end in the initial state  */
 #define NZ_STATUS_TIMEOUT 0x10u    /* a bounded wait on a bulk copy ran out    */
 #define NZ_STATUS_BAD_UNIT 0x20u   /* a unit number of a gather list is out of range */
+#define NZ_STATUS_BAD_INDEX 0x40u  /* nz_mx4_*: a row or matrix number is out of range */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int nz_version(void);
@@ -463,6 +464,52 @@ int nz_peer_alloc(uint64_t bytes, void **ptr, void *handle64);
 int nz_peer_open(const void *handle64, void **ptr);
 int nz_peer_close(void *ptr);
 int nz_peer_free(void *ptr);
+
+/* ---- weights in microscaled 4-bit floating point -------------------------- */
+
+/* A stack of `matrices` matrices [rows, cols].  Every 32 consecutive elements of a
+ * row share a scale, a power of two (one byte, e8m0); an element is four bits (sign,
+ * two exponent bits, one mantissa bit).  The scale is 2^(floor(log2 a) - 2) for the
+ * block's largest magnitude a, not below 2^-127; elements are rounded to the nearest
+ * code, ties to even, and saturate at 6 scales.  A block with an infinity or a NaN
+ * stands for NaN throughout.  Codes: row by row, 16 bytes a block, nz_mx4_code_bytes
+ * in all.  Scales: in the tensor cores' order (described in csrc/nz_mx4.cuh),
+ * nz_mx4_scale_bytes in all.  Both buffers are 16-byte aligned.  Tensors are bf16 or
+ * fp16; rows * matrices and cols stay below 2^31.
+ * Reference: none - it has no quantised storage of its own; its lossy precisions
+ * (cuda/kernels.cuh:53-156) round mantissas and keep entropy-coded exponents. */
+#define NZ_DTYPE_BF16 0
+#define NZ_DTYPE_FP16 1
+
+uint64_t nz_mx4_code_bytes(uint64_t matrices, uint64_t rows, uint64_t cols);
+uint64_t nz_mx4_scale_bytes(uint64_t matrices, uint64_t rows, uint64_t cols);
+int nz_mx4_quantize(const void *in, int dtype, uint64_t matrices, uint64_t rows, uint64_t cols,
+                    void *codes, void *scales, void *stream);
+/* The numbers the codes stand for, rounded to `dtype`. */
+int nz_mx4_dequantize(const void *codes, const void *scales, uint64_t matrices, uint64_t rows,
+                      uint64_t cols, int dtype, void *out, void *stream);
+/* Rows row_list[0..n_list) (int64) of the stack seen as one table of matrices * rows
+ * rows.  A number outside it gives a row of zeros and NZ_STATUS_BAD_INDEX. */
+int nz_mx4_gather_rows(const void *codes, const void *scales, uint64_t matrices, uint64_t rows,
+                       uint64_t cols, int dtype, const void *row_list, uint64_t n_list, void *out,
+                       void *status, void *stream);
+
+/* y[r] = q(x[r / per_input]) q(W[e])^T + bias[e], where q() quantises a row as above,
+ * W[e] is matrix e = experts[r] of the stack (experts = NULL: matrix 0) and bias is
+ * [matrices, rows] or NULL.  x has n_rows / per_input rows, x_stride elements apart
+ * (16-byte aligned rows are read with wide loads); y is [n_rows, rows]; x, bias and y
+ * are of type `dtype`.  Sums are fp32, the bias is added before the one rounding.
+ * experts[r] = -1 gives a row of zeros; any other number outside 0 .. matrices - 1 too,
+ * and sets NZ_STATUS_BAD_INDEX.  The workspace is 256-byte aligned, of
+ * nz_mx4_linear_workspace_bytes bytes for the current device, needs no set-up and is
+ * free again when the call's work is done.  The results do not depend on the order in
+ * which blocks run. */
+uint64_t nz_mx4_linear_workspace_bytes(uint64_t matrices, uint64_t rows, uint64_t cols,
+                                       uint64_t n_rows);
+int nz_mx4_linear(const void *codes, const void *scales, uint64_t matrices, uint64_t rows,
+                  uint64_t cols, int dtype, const void *x, uint64_t x_stride, uint64_t n_rows,
+                  uint64_t per_input, const void *experts, const void *bias, void *y,
+                  void *workspace, uint64_t workspace_bytes, void *status, void *stream);
 
 #ifdef __cplusplus
 }

@@ -4,7 +4,7 @@ the reference's module names (``neuzip.nn``, ``neuzip.ops``, ``neuzip.binding``,
 import sys
 
 import neuzip_b200 as _impl
-from neuzip_b200 import (Algorithm, Manager, binding, compressed_lomo_hook, lomo_hook, nn, ops,
+from neuzip_b200 import (Algorithm, Manager, MX4Manager, binding, compressed_lomo_hook, lomo_hook, nn, ops,
                          utils)
 
 for _name in ("nn", "ops", "binding", "utils", "backend"):
@@ -13,4 +13,4 @@ for _name in ("nn", "ops", "binding", "utils", "backend"):
 sys.modules[__name__ + "._cuda"] = _impl.backend._cuda  # attribute-style stand-in
 _cuda = _impl.backend._cuda
 
-__all__ = ["ops", "nn", "Algorithm", "Manager", "lomo_hook", "compressed_lomo_hook"]
+__all__ = ["ops", "nn", "Algorithm", "Manager", "MX4Manager", "lomo_hook", "compressed_lomo_hook"]

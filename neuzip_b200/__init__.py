@@ -7,9 +7,9 @@ Package root mirrors neuzip/__init__.py:10-35: ``nn``, ``ops``, ``Algorithm``,
 import torch
 
 from . import nn, ops
-from .binding import Algorithm, Manager
+from .binding import Algorithm, Manager, MX4Manager
 
-__all__ = ["ops", "nn", "Algorithm", "Manager", "lomo_hook", "compressed_lomo_hook"]
+__all__ = ["ops", "nn", "Algorithm", "Manager", "MX4Manager", "lomo_hook", "compressed_lomo_hook"]
 __version__ = "0.1.0"
 
 

@@ -222,3 +222,23 @@ class Manager:
 
     def total_size(self) -> int:
         return sum(self.size(h) for h in self.meta_dict)
+
+
+class MX4Manager(Manager):
+    """A manager that holds tensors in microscaled 4-bit floating point (4.25 bits an element,
+    lossy) instead of compressing them, and whose `linear` multiplies the stored form on the
+    tensor cores, inputs quantised on the way (:mod:`neuzip_b200.mx4`).  Same methods as
+    :class:`Manager`; bf16 and fp16 tensors; `read` returns the stored numbers in the type that
+    was written.  Not in the reference."""
+
+    def __init__(self) -> None:
+        from .mx4 import MX4Backend
+        self._be = MX4Backend()
+        self.meta_dict: Dict[str, torch.Size] = {}
+
+    def grouped_linear(self, handle: str, inputs: torch.Tensor, experts: torch.Tensor,
+                       bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Every row of `inputs` times the matrix that `experts` names for it, for a handle that
+        holds a stack of matrices ``[E, out, in]`` (and `bias` ``[E, out]``): ``[T, k]`` expert
+        numbers and ``[T, in]`` or ``[T, k, in]`` inputs give ``[T, k, out]``; -1 gives zeros."""
+        return self._be.grouped_linear(handle, inputs, experts, bias)

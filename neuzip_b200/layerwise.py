@@ -75,6 +75,8 @@ def attach(model: torch.nn.Module, manager,
     weights out.  Larger inputs keep the batched decode."""
     is_block = is_block or default_block_filter
     backend = manager._be
+    if getattr(backend, "multiplies_stored", False):
+        raise ValueError("this manager multiplies by the stored form: there is nothing to decode ahead")
     if fuse_single_token:
         manager.fuse_vector_linear(True)
     _mark_module_list_children(model)

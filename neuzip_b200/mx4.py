@@ -1,0 +1,308 @@
+"""Backend that holds tensors in microscaled 4-bit floating point (MXFP4) and multiplies by
+them as they are: the counterpart of :class:`neuzip_b200.backend.CodecBackend` with the same
+methods, over the ``nz_mx4_*`` calls of ``libneuzip_b200.so``.
+
+Every 32 consecutive elements of the last dimension share a power of two; an element keeps a
+sign, two exponent bits and one mantissa bit, 4.25 bits in all.  `linear` and
+`grouped_linear` quantise their inputs by the same rule, so that the tensor cores multiply
+4-bit operands directly; the weights are never decoded.  The reference has no such form: its
+lossy precisions (cuda/kernels.cuh:53-156) keep entropy-coded exponents and decompress before
+every product (cuda/high_level.cu:252-263).
+"""
+from __future__ import annotations
+
+import functools
+import math
+from dataclasses import dataclass, field
+from typing import Dict, List, Optional, Sequence
+
+import torch
+
+from . import _lib
+from .backend import _ptr
+
+_DTYPES = {torch.bfloat16: _lib.NZ_DTYPE_BF16, torch.float16: _lib.NZ_DTYPE_FP16}
+_NAMES = {torch.bfloat16: "bfloat16", torch.float16: "float16"}
+
+
+@dataclass
+class _Entry:
+    shape: torch.Size
+    dtype: torch.dtype
+    matrices: int             # the stack that is stored: [matrices, rows, cols]
+    rows: int
+    cols: int
+    codes: torch.Tensor       # uint8
+    scales: torch.Tensor      # uint8
+    streams: set = field(default_factory=set)    # streams whose use the allocator knows of
+
+    @property
+    def numel(self) -> int:
+        return self.matrices * self.rows * self.cols
+
+
+def _stack(shape: Sequence[int]):
+    """How a tensor is stored: three dimensions are a stack of matrices, anything else rows."""
+    if len(shape) == 0:
+        return 1, 1, 1
+    if len(shape) == 3:
+        return int(shape[0]), int(shape[1]), int(shape[2])
+    return 1, math.prod(int(d) for d in shape[:-1]), int(shape[-1])
+
+
+@functools.lru_cache(maxsize=512)
+def _sizes(matrices: int, rows: int, cols: int):
+    L = _lib.load()
+    return int(L.nz_mx4_code_bytes(matrices, rows, cols)), int(L.nz_mx4_scale_bytes(matrices, rows, cols))
+
+
+@functools.lru_cache(maxsize=2048)
+def _workspace_bytes(device: int, matrices: int, rows: int, cols: int, n_rows: int) -> int:
+    return int(_lib.load().nz_mx4_linear_workspace_bytes(matrices, rows, cols, n_rows))
+
+
+class MX4Backend:
+    """`read / write / size / linear / linear_without_bias / split` and the extras of the codec
+    backends, on 4-bit storage."""
+
+    supports_operand_order = False
+    multiplies_stored = True           # `linear` never decodes: there is nothing to decode ahead
+
+    def __init__(self) -> None:
+        self._lib = _lib.load()
+        self._cache: Dict[str, _Entry] = {}
+        self._status: Dict[int, torch.Tensor] = {}
+
+    # -- helpers ---------------------------------------------------------
+    def _status_of(self, device: int) -> torch.Tensor:
+        word = self._status.get(device)
+        if word is None:
+            _lib.check(self._lib.nz_device_check())
+            word = self._status[device] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+        return word
+
+    def status(self) -> int:
+        """Status word accumulated so far, over all devices (synchronises)."""
+        bits = 0
+        for word in list(self._status.values()):
+            bits |= int(word.item()) & 0xFFFFFFFF
+        return bits
+
+    def check(self) -> None:
+        word = self.status()
+        if word:
+            raise _lib.NeuzipError("a kernel reported: " + _lib.describe_status(word))
+
+    def _get(self, name: str) -> _Entry:
+        entry = self._cache.get(name)
+        if entry is None:
+            raise RuntimeError("Data not found")
+        return entry
+
+    def _use(self, entry: _Entry) -> int:
+        """The current stream of the current device, which must be the entry's; from now on
+        the allocator does not hand the entry's memory out while that stream may read it."""
+        device = entry.codes.get_device()
+        stream = torch._C._cuda_getCurrentRawStream(device)
+        if stream not in entry.streams:
+            current = torch.cuda.current_stream(device)
+            entry.codes.record_stream(current)
+            entry.scales.record_stream(current)
+            entry.streams.add(stream)
+        return stream
+
+    # -- the six methods of the extension class ----------------------------
+    def write(self, name: str, tensor: torch.Tensor) -> None:
+        """Quantise `tensor` (bf16 or fp16, any shape; three dimensions are a stack of matrices)
+        and keep it under `name`, on its own device (a CPU tensor goes to the current one)."""
+        if tensor.dtype not in _DTYPES:
+            raise RuntimeError("Unsupported data type")
+        if not tensor.is_cuda:
+            tensor = tensor.cuda()
+        source = tensor.detach().contiguous()
+        device = source.get_device()
+        matrices, rows, cols = _stack(source.shape)
+        with torch.cuda.device(device):
+            self._status_of(device)
+            code_bytes, scale_bytes = _sizes(matrices, rows, cols)
+            codes = torch.empty(code_bytes, dtype=torch.uint8, device=source.device)
+            # the last row tile's missing rows are never used, but they are part of a checkpoint
+            scales = (torch.zeros if rows % 128 else torch.empty)(
+                scale_bytes, dtype=torch.uint8, device=source.device)
+            stream = torch._C._cuda_getCurrentRawStream(device)
+            _lib.check(self._lib.nz_mx4_quantize(_ptr(source), _DTYPES[tensor.dtype], matrices, rows, cols,
+                                                 _ptr(codes), _ptr(scales), stream))
+        self._cache[name] = _Entry(tensor.shape, tensor.dtype, matrices, rows, cols, codes, scales,
+                                   {stream})
+
+    def read(self, name: str) -> torch.Tensor:
+        """The stored numbers as a flat tensor of the type that was written."""
+        entry = self._get(name)
+        return self.read_shaped(name, (entry.numel,))
+
+    def read_shaped(self, name: str, shape) -> torch.Tensor:
+        entry = self._get(name)
+        with torch.cuda.device(entry.codes.device):
+            out = torch.empty(entry.numel, dtype=entry.dtype, device=entry.codes.device).view(tuple(shape))
+            _lib.check(self._lib.nz_mx4_dequantize(
+                _ptr(entry.codes), _ptr(entry.scales), entry.matrices, entry.rows, entry.cols,
+                _DTYPES[entry.dtype], _ptr(out), self._use(entry)))
+        return out
+
+    def read_many(self, names: Sequence[str]) -> List[torch.Tensor]:
+        return [self.read(name) for name in names]
+
+    def read_rows(self, name: str, rows: torch.Tensor, row_len: int) -> torch.Tensor:
+        """Rows ``rows`` (any integer tensor) of the stored tensor seen as a
+        ``[numel / row_len, row_len]`` table.  A row outside the table reads as zeros and raises
+        at the next ``check()``."""
+        entry = self._get(name)
+        if row_len <= 0 or entry.numel % row_len:
+            raise ValueError(f"row length {row_len} does not divide the {entry.numel} stored elements")
+        if rows.is_floating_point() or rows.is_complex() or rows.dtype == torch.bool:
+            raise TypeError(f"row numbers must be integers, got {rows.dtype}")
+        device = entry.codes.device
+        rows = rows.reshape(-1).to(device=device, dtype=torch.int64).contiguous()
+        if row_len != entry.cols:
+            # rows of several dimensions: each is a run of the table's own rows
+            if row_len % entry.cols:
+                raise ValueError(f"row length {row_len} is not a whole number of stored rows")
+            run = row_len // entry.cols
+            rows = (rows.unsqueeze(1) * run + torch.arange(run, device=device)).reshape(-1)
+        with torch.cuda.device(device):
+            out = torch.empty(rows.numel(), entry.cols, dtype=entry.dtype, device=device)
+            _lib.check(self._lib.nz_mx4_gather_rows(
+                _ptr(entry.codes), _ptr(entry.scales), entry.matrices, entry.rows, entry.cols,
+                _DTYPES[entry.dtype], _ptr(rows), rows.numel(), _ptr(out),
+                _ptr(self._status_of(device.index)), self._use(entry)))
+        return out.view(-1, row_len)
+
+    def size(self, name: str) -> int:
+        """Stored bytes, 0 for an unknown name."""
+        entry = self._cache.get(name)
+        return 0 if entry is None else entry.codes.numel() + entry.scales.numel()
+
+    def linear(self, name: str, input: torch.Tensor, shape: Sequence[int],
+               bias: Optional[torch.Tensor]) -> torch.Tensor:
+        """``q(input) @ q(W)^T (+ bias)``: the inputs are quantised like the weights, sums are
+        fp32, the result is rounded once to the type of `input`."""
+        entry = self._get(name)
+        if len(shape) != 2 or entry.matrices != 1 or int(shape[0]) * int(shape[1]) != entry.numel \
+                or int(shape[1]) != entry.cols:
+            raise ValueError(f"linear needs a matrix, got a tensor of shape {tuple(shape)}")
+        x = self._checked_input(entry, input, bias)
+        n_rows = x.shape[0]
+        y = torch.empty(input.shape[:-1] + (entry.rows,), dtype=input.dtype, device=input.device)
+        self._launch(entry, x, n_rows, 1, None, bias, y)
+        return y
+
+    def linear_without_bias(self, name: str, input: torch.Tensor, shape: Sequence[int]) -> torch.Tensor:
+        return self.linear(name, input, shape, None)
+
+    def grouped_linear(self, name: str, input: torch.Tensor, experts: torch.Tensor,
+                       bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Row ``r`` of the result is ``q(input[r]) @ q(W[experts[r]])^T (+ bias[experts[r]])`` for a
+        stack ``W`` of matrices.  `experts` is an integer tensor; `input` has its shape and one
+        more dimension, or lacks its last one, and then every input row goes to all the
+        experts named for it: ``[T, k]`` experts and ``[T, in]`` inputs give ``[T, k, out]``.
+        -1 means no expert and gives a row of zeros; other numbers outside the stack too, and
+        they raise at the next ``check()``.  Nothing synchronises with the host."""
+        entry = self._get(name)
+        if len(entry.shape) != 3:
+            raise ValueError("grouped_linear needs a stack of matrices (three dimensions), "
+                             f"got a tensor of shape {tuple(entry.shape)}")
+        if experts.is_floating_point() or experts.is_complex() or experts.dtype == torch.bool:
+            raise TypeError(f"expert numbers must be integers, got {experts.dtype}")
+        if experts.device != entry.codes.device:
+            raise ValueError(f"expert numbers are on {experts.device}, the weights on {entry.codes.device}")
+        lead, per_input = input.shape[:-1], 1
+        if lead != experts.shape:
+            if experts.dim() == 0 or lead != experts.shape[:-1]:
+                raise ValueError(f"inputs of shape {tuple(input.shape)} do not match experts of shape "
+                                 f"{tuple(experts.shape)}")
+            per_input = int(experts.shape[-1])
+        x = self._checked_input(entry, input, bias)
+        ids = experts.to(torch.int64).contiguous()
+        y = torch.empty(experts.shape + (entry.rows,), dtype=input.dtype, device=input.device)
+        self._launch(entry, x, ids.numel(), per_input, ids, bias, y)
+        return y
+
+    def _checked_input(self, entry: _Entry, input: torch.Tensor,
+                       bias: Optional[torch.Tensor]) -> torch.Tensor:
+        """`input` as rows one element apart inside, after the checks the products share."""
+        if input.dtype not in _DTYPES:
+            raise RuntimeError("Unsupported data type")
+        if input.dim() < 1 or input.shape[-1] != entry.cols or entry.cols == 0:
+            raise ValueError(f"inputs of shape {tuple(input.shape)} do not fit weights of shape "
+                             f"{tuple(entry.shape)}")
+        if input.device != entry.codes.device:
+            raise ValueError(f"inputs are on {input.device}, the weights on {entry.codes.device}")
+        if bias is not None and (bias.dtype != input.dtype or bias.device != input.device
+                                 or bias.numel() != entry.matrices * entry.rows):
+            raise ValueError(f"bias must be {entry.matrices * entry.rows} numbers of type "
+                             f"{_NAMES[input.dtype]} on {input.device}")
+        if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
+            raise RuntimeError("products with 4-bit weights have no gradient here: use nn.Linear, or "
+                               "call under torch.no_grad()")
+        x = input.reshape(-1, entry.cols) if input.dim() != 2 else input
+        if x.stride(1) != 1 or x.stride(0) < entry.cols:
+            x = x.contiguous()
+        return x
+
+    def _launch(self, entry: _Entry, x: torch.Tensor, n_rows: int, per_input: int,
+                ids: Optional[torch.Tensor], bias: Optional[torch.Tensor], y: torch.Tensor) -> None:
+        if y.numel() == 0:
+            return
+        device = x.get_device()
+        if device != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return self._launch(entry, x, n_rows, per_input, ids, bias, y)
+        if bias is not None:
+            bias = bias.contiguous()
+        # from the allocator on every call: calls on other streams and captured graphs have their own
+        workspace = torch.empty(_workspace_bytes(device, entry.matrices, entry.rows, entry.cols, n_rows),
+                                dtype=torch.uint8, device=x.device)
+        rc = self._lib.nz_mx4_linear(
+            _ptr(entry.codes), _ptr(entry.scales), entry.matrices, entry.rows, entry.cols,
+            _DTYPES[x.dtype], _ptr(x), x.stride(0), n_rows, per_input, _ptr(ids), _ptr(bias), _ptr(y),
+            _ptr(workspace), workspace.numel(), _ptr(self._status_of(device)), self._use(entry))
+        if rc:
+            _lib.check(rc)
+
+    def split(self, tensor: torch.Tensor):
+        raise NotImplementedError("4-bit storage has no split()")
+
+    # -- serialisation ----------------------------------------------------
+    def export_entry(self, name: str) -> dict:
+        """The stored form of one tensor as CPU tensors plus what is needed to read it."""
+        e = self._cache[name]
+        return {"format": "MXFP4", "dtype": _NAMES[e.dtype], "stack": (e.matrices, e.rows, e.cols),
+                "codes": e.codes.cpu(), "scales": e.scales.cpu()}
+
+    def import_entry(self, name: str, blob: dict) -> None:
+        """Inverse of `export_entry`: the stored bytes go straight to the GPU."""
+        if blob.get("format") != "MXFP4":
+            raise ValueError(f"checkpoint entry does not match this manager (format {blob.get('format')!r})")
+        shape = torch.Size(blob["shape"])
+        stack = _stack(shape)
+        dtype = {v: k for k, v in _NAMES.items()}.get(blob["dtype"])
+        if dtype is None or tuple(blob["stack"]) != stack:
+            raise ValueError("checkpoint entry: type or shape does not fit the stored bytes")
+        if (blob["codes"].numel(), blob["scales"].numel()) != _sizes(*stack):
+            raise ValueError("checkpoint entry: codes or scales have the wrong length")
+        codes = blob["codes"].to(device="cuda", dtype=torch.uint8).contiguous()
+        scales = blob["scales"].to(device="cuda", dtype=torch.uint8).contiguous()
+        device = codes.get_device()
+        self._status_of(device)
+        self._cache[name] = _Entry(shape, dtype, *stack, codes, scales,
+                                   {torch._C._cuda_getCurrentRawStream(device)})
+
+    # -- extras -----------------------------------------------------------
+    def erase(self, name: str) -> None:
+        self._cache.pop(name, None)
+
+    def entry(self, name: str) -> _Entry:
+        return self._cache[name]
+
+    def names(self):
+        return list(self._cache)
