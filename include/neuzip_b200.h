@@ -472,27 +472,25 @@ int nz_peer_free(void *ptr);
  * two exponent bits, one mantissa bit).  The scale is 2^(floor(log2 a) - 2) for the
  * block's largest magnitude a, not below 2^-127; elements are rounded to the nearest
  * code, ties to even, and saturate at 6 scales.  A block with an infinity or a NaN
- * stands for NaN throughout.  Codes: row by row, 16 bytes a block, nz_mx4_code_bytes
- * in all.  Scales: in the tensor cores' order (described in csrc/nz_mx4.cuh),
- * nz_mx4_scale_bytes in all.  Both buffers are 16-byte aligned.  Tensors are bf16 or
- * fp16; rows * matrices and cols stay below 2^31.
+ * stands for NaN throughout.  The stored bytes (nz_mx4_bytes, 16-byte aligned) are in
+ * the order the tensor cores take, described in csrc/nz_mx4.cuh; rows are filled up to
+ * a multiple of 128 per matrix, columns to one of 32.  Tensors are bf16 or fp16;
+ * rows * matrices and cols stay below 2^31.
  * Reference: none - it has no quantised storage of its own; its lossy precisions
  * (cuda/kernels.cuh:53-156) round mantissas and keep entropy-coded exponents. */
 #define NZ_DTYPE_BF16 0
 #define NZ_DTYPE_FP16 1
 
-uint64_t nz_mx4_code_bytes(uint64_t matrices, uint64_t rows, uint64_t cols);
-uint64_t nz_mx4_scale_bytes(uint64_t matrices, uint64_t rows, uint64_t cols);
+uint64_t nz_mx4_bytes(uint64_t matrices, uint64_t rows, uint64_t cols);
 int nz_mx4_quantize(const void *in, int dtype, uint64_t matrices, uint64_t rows, uint64_t cols,
-                    void *codes, void *scales, void *stream);
+                    void *packed, void *stream);
 /* The numbers the codes stand for, rounded to `dtype`. */
-int nz_mx4_dequantize(const void *codes, const void *scales, uint64_t matrices, uint64_t rows,
-                      uint64_t cols, int dtype, void *out, void *stream);
+int nz_mx4_dequantize(const void *packed, uint64_t matrices, uint64_t rows, uint64_t cols, int dtype,
+                      void *out, void *stream);
 /* Rows row_list[0..n_list) (int64) of the stack seen as one table of matrices * rows
  * rows.  A number outside it gives a row of zeros and NZ_STATUS_BAD_INDEX. */
-int nz_mx4_gather_rows(const void *codes, const void *scales, uint64_t matrices, uint64_t rows,
-                       uint64_t cols, int dtype, const void *row_list, uint64_t n_list, void *out,
-                       void *status, void *stream);
+int nz_mx4_gather_rows(const void *packed, uint64_t matrices, uint64_t rows, uint64_t cols, int dtype,
+                       const void *row_list, uint64_t n_list, void *out, void *status, void *stream);
 
 /* y[r] = q(x[r / per_input]) q(W[e])^T + bias[e], where q() quantises a row as above,
  * W[e] is matrix e = experts[r] of the stack (experts = NULL: matrix 0) and bias is
@@ -506,10 +504,10 @@ int nz_mx4_gather_rows(const void *codes, const void *scales, uint64_t matrices,
  * which blocks run. */
 uint64_t nz_mx4_linear_workspace_bytes(uint64_t matrices, uint64_t rows, uint64_t cols,
                                        uint64_t n_rows);
-int nz_mx4_linear(const void *codes, const void *scales, uint64_t matrices, uint64_t rows,
-                  uint64_t cols, int dtype, const void *x, uint64_t x_stride, uint64_t n_rows,
-                  uint64_t per_input, const void *experts, const void *bias, void *y,
-                  void *workspace, uint64_t workspace_bytes, void *status, void *stream);
+int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t rows, uint64_t cols, int dtype,
+                  const void *x, uint64_t x_stride, uint64_t n_rows, uint64_t per_input,
+                  const void *experts, const void *bias, void *y, void *workspace,
+                  uint64_t workspace_bytes, void *status, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,92 +1,116 @@
 // Weights in microscaled 4-bit floating point: quantisation, the way back, row lookup.
-// The format is described in nz_mx4.cuh.
+// Format and storage are described in nz_mx4.cuh.
 #include "nz_mx4.cuh"
 
 namespace nz {
 
 constexpr int kMxThreads = 256;
 
-// One warp per (row, step) of the stack, in a grid-stride loop.
-template <typename T, bool VEC>
+// A thread takes a block, a warp eight rows of four blocks: its loads are whole sectors, its stores
+// 128 bytes in a piece.  Warps take items (eight rows, 128 columns) in a grid-stride loop; the rows
+// that fill up the last tile are items too.
+template <typename T, int WIDE>
 __global__ void __launch_bounds__(kMxThreads)
-mx4_quantize_kernel(const T *__restrict__ in, MxShape s, uint8_t *__restrict__ codes,
-                    uint8_t *__restrict__ scales) {
+mx4_quantize_kernel(const T *__restrict__ in, MxShape s, uint8_t *__restrict__ packed) {
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
-  const uint64_t steps = s.steps(), pitch = s.code_pitch(), total = s.matrices * s.rows * steps;
-  for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total;
-       w += warps) {
-    const uint64_t row = w / steps, step = w - row * steps;
-    const uint64_t col = step * kMxStep + lane * 8;
-    float v[8];
-    mx_load8<T, VEC>(in + row * s.cols + col, (int64_t)s.cols - (int64_t)col, v);
-    uint32_t code, byte;
-    mx_quantize8(v, code, byte);
-    if (col / 2 < pitch) *reinterpret_cast<uint32_t *>(codes + row * pitch + col / 2) = code;
+  const uint32_t halves = 2 * (uint32_t)s.steps(), blocks = (uint32_t)s.blocks();
+  const uint32_t tile_groups = (uint32_t)s.row_tiles() * (kMxTileRows / 8);
+  const uint64_t tile_bytes = s.tile_bytes(), total = s.matrices * tile_groups * halves;
+  for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
+    const uint64_t group = w / halves;
+    const uint32_t half = (uint32_t)(w - group * halves), block = half * 4 + (lane >> 3);
+    const uint64_t matrix = group / tile_groups;
+    const uint32_t row = (uint32_t)(group - matrix * tile_groups) * 8 + (lane & 7u);
+    uint32_t v[16], code[4], byte;
+    const int64_t left = row < s.rows ? (int64_t)s.cols - (int64_t)block * kMxBlock : 0;
+    mx_load_block<WIDE>(in + (matrix * s.rows + row) * s.cols + (uint64_t)block * kMxBlock, left, v);
+    mx_quantize_block<T>(v, code, byte);
+    uint8_t *step = packed + (matrix * s.row_tiles() + row / kMxTileRows) * tile_bytes +
+                    (uint64_t)(half >> 1) * kMxStepBytes;
+    const uint32_t r = row % kMxTileRows, first = (half >> 1) * 8;
+    if (block < blocks)
+      *reinterpret_cast<uint4 *>(step + (block - first) * kMxBlockBytes + r * 16) =
+          make_uint4(code[0], code[1], code[2], code[3]);
     const uint32_t word = mx_pack_scales(byte, lane);
-    if ((lane & 15u) == 0) {
-      const uint64_t matrix = row / s.rows, r = row - matrix * s.rows;
-      const uint64_t tile = matrix * s.row_tiles() + r / kMxTileRows;
-      *reinterpret_cast<uint32_t *>(scales + (tile * steps + step) * (2 * kMxChunk) +
-                                    mx_scale_offset((uint32_t)(r % kMxTileRows), lane >> 2, 1)) = word;
+    if (lane < 8) {
+      const uint32_t held = blocks - first < 8 ? blocks - first : 8;
+      *reinterpret_cast<uint32_t *>(step + held * kMxBlockBytes + mx_scale_offset(r, (half & 1) * 4, 1)) = word;
     }
   }
 }
 
-// The way back: one warp per (row, step).  With a list, output row i is row list[i] of the stack
-// (zeros and a status bit where there is no such row).
-template <typename T, bool VEC>
+// The way back, the same items.  With a list, output row i is row list[i] of the stack (zeros and a
+// status bit where there is no such row).
+template <typename T, int WIDE>
 __global__ void __launch_bounds__(kMxThreads)
-mx4_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, MxShape s,
-                      const int64_t *__restrict__ list, uint64_t out_rows, T *__restrict__ out,
-                      uint32_t *status) {
+mx4_dequantize_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64_t *__restrict__ list,
+                      uint64_t out_rows, T *__restrict__ out, uint32_t *status) {
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
-  const uint64_t steps = s.steps(), pitch = s.code_pitch(), total = out_rows * steps;
-  for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total;
-       w += warps) {
-    const uint64_t to = w / steps, step = w - to * steps;
-    const uint64_t col = step * kMxStep + lane * 8;
-    if (col >= s.cols) continue;
+  const uint32_t blocks = (uint32_t)s.blocks(), quads = (blocks + 3) / 4;
+  const uint64_t tile_bytes = s.tile_bytes(), total = (out_rows + 7) / 8 * quads;
+  for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
+    const uint64_t group = w / quads, to = group * 8 + (lane & 7u);
+    const uint32_t block = (uint32_t)(w - group * quads) * 4 + (lane >> 3);
+    if (block >= blocks || to >= out_rows) continue;
     uint64_t row = to;
-    uint32_t code = 0, byte = 0;
     bool there = true;
     if (list) {
       const int64_t want = list[to];
       there = want >= 0 && (uint64_t)want < s.matrices * s.rows;
       row = there ? (uint64_t)want : 0;
-      if (!there && lane == 0 && step == 0 && status) atomicOr(status, NZ_STATUS_BAD_INDEX);
+      if (!there && block == 0 && status) atomicOr(status, NZ_STATUS_BAD_INDEX);
     }
+    uint4 code = make_uint4(0, 0, 0, 0);
+    uint32_t byte = 0;
     if (there) {
-      const uint64_t matrix = row / s.rows, r = row - matrix * s.rows;
-      const uint64_t tile = matrix * s.row_tiles() + r / kMxTileRows;
-      code = *reinterpret_cast<const uint32_t *>(codes + row * pitch + col / 2);
-      byte = scales[(tile * steps + step) * (2 * kMxChunk) +
-                    mx_scale_offset((uint32_t)(r % kMxTileRows), lane >> 2, 1)];
+      const uint64_t matrix = s.matrices == 1 ? 0 : row / s.rows;
+      const uint32_t r = (uint32_t)(row - matrix * s.rows), first = block & ~7u;
+      const uint8_t *step = packed + (matrix * s.row_tiles() + r / kMxTileRows) * tile_bytes +
+                            (uint64_t)(block >> 3) * kMxStepBytes;
+      const uint32_t held = blocks - first < 8 ? blocks - first : 8;
+      code = __ldg(reinterpret_cast<const uint4 *>(step + (block - first) * kMxBlockBytes +
+                                                   (r % kMxTileRows) * 16));
+      byte = __ldg(step + held * kMxBlockBytes + mx_scale_offset(r % kMxTileRows, block & 7u, 1));
     }
     const float scale = mx_scale(byte);
-    T e[8];
+    const uint32_t c[4] = {code.x, code.y, code.z, code.w};
+    T *dst = out + to * s.cols + (uint64_t)block * kMxBlock;
+    const uint64_t left = s.cols - (uint64_t)block * kMxBlock;
+    uint32_t v[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = mx_decode2((code >> (8 * i)) & 255u);
-      e[2 * i] = from_float<T>(f.x * scale);
-      e[2 * i + 1] = from_float<T>(f.y * scale);
+    for (int i = 0; i < 16; ++i) {
+      const float2 f = mx_decode2((c[i / 4] >> (8 * (i & 3))) & 255u);
+      T e[2] = {from_float<T>(f.x * scale), from_float<T>(f.y * scale)};
+      memcpy(&v[i], e, 4);
     }
-    T *dst = out + to * s.cols + col;
-    if (VEC) {
-      uint4 raw;
-      memcpy(&raw, e, 16);
-      *reinterpret_cast<uint4 *>(dst) = raw;
+    if (WIDE == 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (left > 16 * h)
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 16 * h),
+                       "r"(v[8 * h]), "r"(v[8 * h + 1]), "r"(v[8 * h + 2]), "r"(v[8 * h + 3]),
+                       "r"(v[8 * h + 4]), "r"(v[8 * h + 5]), "r"(v[8 * h + 6]), "r"(v[8 * h + 7])
+                       : "memory");
+    } else if (WIDE == 1) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        if (left > 8 * h)
+          *reinterpret_cast<uint4 *>(dst + 8 * h) = make_uint4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < s.cols) dst[i] = e[i];
+      for (int i = 0; i < 32; ++i)
+        if (i < left) {
+          const uint16_t bits = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+          memcpy(dst + i, &bits, 2);
+        }
     }
   }
 }
 
 bool mx_shape(const char *who, uint64_t matrices, uint64_t rows, uint64_t cols) {
-  // 32-bit row numbers in the product, byte offsets in 64 bits
+  // 32-bit row and block numbers, byte offsets in 64 bits
   if (cols >= (1ull << 31) || rows >= (1ull << 31) || matrices >= (1ull << 31) ||
       matrices * rows >= (1ull << 31)) {
     set_error("%s: a stack of %llu matrices [%llu, %llu] has 2^31 or more rows or columns", who,
@@ -102,95 +126,96 @@ bool mx_dtype(const char *who, int dtype) {
 }
 static unsigned mx_grid(uint64_t warps) {
   const uint64_t blocks = (warps + kMxThreads / 32 - 1) / (kMxThreads / 32);
-  const uint64_t most = (uint64_t)sm_count() * 8;            // 2048 threads an SM, twice over
+  const uint64_t most = (uint64_t)sm_count() * 8;            // 2048 threads an SM
   return (unsigned)(blocks < most ? blocks : most);
+}
+// How wide the rows of a contiguous tensor can be read or written.
+static int mx_wide(const void *p, uint64_t cols) {
+  return cols % 16 == 0 && ((uintptr_t)p & 31) == 0 ? 2 : cols % 8 == 0 && ((uintptr_t)p & 15) == 0 ? 1 : 0;
 }
 
 }  // namespace nz
 
-extern "C" uint64_t nz_mx4_code_bytes(uint64_t matrices, uint64_t rows, uint64_t cols) {
-  return matrices * rows * nz::MxShape{matrices, rows, cols}.code_pitch();
+extern "C" uint64_t nz_mx4_bytes(uint64_t matrices, uint64_t rows, uint64_t cols) {
+  return nz::MxShape{matrices, rows, cols}.bytes();
 }
 
-extern "C" uint64_t nz_mx4_scale_bytes(uint64_t matrices, uint64_t rows, uint64_t cols) {
-  const nz::MxShape s{matrices, rows, cols};
-  return matrices * s.row_tiles() * s.steps() * 2 * nz::kMxChunk;
-}
-
-extern "C" int nz_mx4_quantize(const void *in, int dtype, uint64_t matrices, uint64_t rows,
-                               uint64_t cols, void *codes, void *scales, void *stream) {
+template <typename T>
+static int quantize(const void *in, const nz::MxShape &s, void *packed, cudaStream_t st) {
   using namespace nz;
-  if (!mx_dtype("nz_mx4_quantize", dtype) || !mx_shape("nz_mx4_quantize", matrices, rows, cols))
-    return NZ_E_ARG;
-  const MxShape s{matrices, rows, cols};
-  const uint64_t warps = matrices * rows * s.steps();
-  if (warps == 0) return NZ_OK;
-  if (!in || !codes || !scales || ((uintptr_t)in & 1) || ((uintptr_t)codes & 15) ||
-      ((uintptr_t)scales & 15)) {
-    set_error("nz_mx4_quantize: null or misaligned pointer (codes and scales 16-byte aligned)");
-    return NZ_E_ARG;
-  }
-  const bool vec = cols % 8 == 0 && ((uintptr_t)in & 15) == 0;
-  cudaStream_t st = (cudaStream_t)stream;
-#define NZ_MX_GO(T, VEC)                                                                          \
-  mx4_quantize_kernel<T, VEC><<<mx_grid(warps), kMxThreads, 0, st>>>((const T *)in, s,            \
-                                                                     (uint8_t *)codes, (uint8_t *)scales)
-  if (dtype == NZ_DTYPE_BF16) {
-    if (vec) NZ_MX_GO(__nv_bfloat16, true); else NZ_MX_GO(__nv_bfloat16, false);
-  } else {
-    if (vec) NZ_MX_GO(__half, true); else NZ_MX_GO(__half, false);
-  }
-#undef NZ_MX_GO
+  const uint64_t warps = s.matrices * s.row_tiles() * (kMxTileRows / 8) * 2 * s.steps();
+  const int wide = mx_wide(in, s.cols);
+  auto kern = wide == 2 ? mx4_quantize_kernel<T, 2> : wide == 1 ? mx4_quantize_kernel<T, 1>
+                                                                : mx4_quantize_kernel<T, 0>;
+  kern<<<mx_grid(warps), kMxThreads, 0, st>>>((const T *)in, s, (uint8_t *)packed);
   NZ_LAUNCH_CHECK("mx4_quantize_kernel");
   return NZ_OK;
 }
 
-static int mx4_dequantize(const char *who, const void *codes, const void *scales, uint64_t matrices,
-                          uint64_t rows, uint64_t cols, int dtype, const int64_t *list,
-                          uint64_t out_rows, void *out, void *status, void *stream) {
+extern "C" int nz_mx4_quantize(const void *in, int dtype, uint64_t matrices, uint64_t rows,
+                               uint64_t cols, void *packed, void *stream) {
   using namespace nz;
-  if (!mx_dtype(who, dtype) || !mx_shape(who, matrices, rows, cols)) return NZ_E_ARG;
+  if (!mx_dtype("nz_mx4_quantize", dtype) || !mx_shape("nz_mx4_quantize", matrices, rows, cols))
+    return NZ_E_ARG;
   const MxShape s{matrices, rows, cols};
-  const uint64_t warps = out_rows * s.steps();
-  if (warps == 0) return NZ_OK;
-  if (out_rows >= (1ull << 40)) {
-    set_error("%s: too many rows", who);
+  if (s.bytes() == 0) return NZ_OK;
+  if (!in || !packed || ((uintptr_t)in & 1) || ((uintptr_t)packed & 15)) {
+    set_error("nz_mx4_quantize: null or misaligned pointer (stored bytes 16-byte aligned)");
     return NZ_E_ARG;
   }
-  const bool held = matrices * rows > 0;       // a list may name rows of an empty table: all are bad
-  if ((held && (!codes || !scales)) || !out || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15) ||
-      ((uintptr_t)out & 1) || ((uintptr_t)list & 7)) {
-    set_error("%s: null or misaligned pointer (codes and scales 16-byte aligned)", who);
-    return NZ_E_ARG;
-  }
-  const bool vec = cols % 8 == 0 && ((uintptr_t)out & 15) == 0;
-  cudaStream_t st = (cudaStream_t)stream;
-#define NZ_MX_GO(T, VEC)                                                                     \
-  mx4_dequantize_kernel<T, VEC><<<mx_grid(warps), kMxThreads, 0, st>>>(                      \
-      (const uint8_t *)codes, (const uint8_t *)scales, s, list, out_rows, (T *)out, (uint32_t *)status)
-  if (dtype == NZ_DTYPE_BF16) {
-    if (vec) NZ_MX_GO(__nv_bfloat16, true); else NZ_MX_GO(__nv_bfloat16, false);
-  } else {
-    if (vec) NZ_MX_GO(__half, true); else NZ_MX_GO(__half, false);
-  }
-#undef NZ_MX_GO
+  return dtype == NZ_DTYPE_BF16 ? quantize<__nv_bfloat16>(in, s, packed, (cudaStream_t)stream)
+                                : quantize<__half>(in, s, packed, (cudaStream_t)stream);
+}
+
+template <typename T>
+static int dequantize(const void *packed, const nz::MxShape &s, const void *list, uint64_t out_rows,
+                      void *out, void *status, cudaStream_t st) {
+  using namespace nz;
+  const uint64_t warps = (out_rows + 7) / 8 * ((s.blocks() + 3) / 4);
+  const int wide = mx_wide(out, s.cols);
+  auto kern = wide == 2 ? mx4_dequantize_kernel<T, 2> : wide == 1 ? mx4_dequantize_kernel<T, 1>
+                                                                  : mx4_dequantize_kernel<T, 0>;
+  kern<<<mx_grid(warps), kMxThreads, 0, st>>>((const uint8_t *)packed, s, (const int64_t *)list, out_rows,
+                                              (T *)out, (uint32_t *)status);
   NZ_LAUNCH_CHECK("mx4_dequantize_kernel");
   return NZ_OK;
 }
 
-extern "C" int nz_mx4_dequantize(const void *codes, const void *scales, uint64_t matrices,
-                                 uint64_t rows, uint64_t cols, int dtype, void *out, void *stream) {
-  return mx4_dequantize("nz_mx4_dequantize", codes, scales, matrices, rows, cols, dtype, nullptr,
-                        matrices * rows, out, nullptr, stream);
+static int dequantize_checked(const char *who, const void *packed, uint64_t matrices, uint64_t rows,
+                              uint64_t cols, int dtype, const void *list, uint64_t out_rows, void *out,
+                              void *status, void *stream) {
+  using namespace nz;
+  if (!mx_dtype(who, dtype) || !mx_shape(who, matrices, rows, cols)) return NZ_E_ARG;
+  const MxShape s{matrices, rows, cols};
+  if (out_rows == 0 || cols == 0) return NZ_OK;
+  if (out_rows >= (1ull << 40)) {
+    set_error("%s: too many rows", who);
+    return NZ_E_ARG;
+  }
+  // a list may name rows of an empty table: none of them exists
+  if ((s.bytes() && !packed) || !out || ((uintptr_t)packed & 15) || ((uintptr_t)out & 1) ||
+      ((uintptr_t)list & 7)) {
+    set_error("%s: null or misaligned pointer (stored bytes 16-byte aligned)", who);
+    return NZ_E_ARG;
+  }
+  return dtype == NZ_DTYPE_BF16
+             ? dequantize<__nv_bfloat16>(packed, s, list, out_rows, out, status, (cudaStream_t)stream)
+             : dequantize<__half>(packed, s, list, out_rows, out, status, (cudaStream_t)stream);
 }
 
-extern "C" int nz_mx4_gather_rows(const void *codes, const void *scales, uint64_t matrices,
-                                  uint64_t rows, uint64_t cols, int dtype, const void *row_list,
-                                  uint64_t n_list, void *out, void *status, void *stream) {
+extern "C" int nz_mx4_dequantize(const void *packed, uint64_t matrices, uint64_t rows, uint64_t cols,
+                                 int dtype, void *out, void *stream) {
+  return dequantize_checked("nz_mx4_dequantize", packed, matrices, rows, cols, dtype, nullptr,
+                            matrices * rows, out, nullptr, stream);
+}
+
+extern "C" int nz_mx4_gather_rows(const void *packed, uint64_t matrices, uint64_t rows, uint64_t cols,
+                                  int dtype, const void *row_list, uint64_t n_list, void *out,
+                                  void *status, void *stream) {
   if (n_list && !row_list) {
     nz::set_error("nz_mx4_gather_rows: null row list");
     return NZ_E_ARG;
   }
-  return mx4_dequantize("nz_mx4_gather_rows", codes, scales, matrices, rows, cols, dtype,
-                        (const int64_t *)row_list, n_list, out, status, stream);
+  return dequantize_checked("nz_mx4_gather_rows", packed, matrices, rows, cols, dtype, row_list, n_list,
+                            out, status, stream);
 }

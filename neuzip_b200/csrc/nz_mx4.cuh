@@ -8,11 +8,14 @@
 // so that a / s lies in [4, 8).  A block that holds an infinity or a NaN has the scale byte 255
 // and stands for NaN throughout.  Element 2j of a row is the low half of byte j.
 //
-// Codes lie row by row, 16 bytes a block.  Scales lie as the tensor cores take them: for a tile of
-// 128 rows and 128 columns 512 bytes, of which row r, block b of the four has byte
-// (r % 32) * 16 + (r / 32) * 4 + b; the two halves of 256 columns (a "step" of the product) follow
-// each other, then the steps of a row tile, then the row tiles.  The blocks that fill the last step
-// have the scale byte 0.  Every matrix of a stack begins a row tile of its own.
+// Storage is the order in which the tensor cores take operands from shared memory, so that a
+// product fetches whole runs of it.  A matrix is cut into tiles of 128 rows (the last one is filled
+// up with zeros), a tile into steps of 256 columns.  A step lies in one piece: its blocks, one
+// after the other, each with 16 bytes for every row of the tile, then its scales.  These are two
+// chunks, one for each 128 columns, of 512 bytes in which row r, block b of four has byte
+// (r % 32) * 16 + (r / 32) * 4 + b.  The last step has as many blocks as there are; scales of
+// blocks that do not exist are 0.  Inputs of a product lie the same way in tiles of another number
+// of rows, with all eight blocks in every step and a pair of chunks for every 128 rows.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -29,10 +32,17 @@ constexpr uint32_t kMxChunk = 512;           // scales of 128 rows x 128 columns
 
 struct MxShape {
   uint64_t matrices, rows, cols;
-  __host__ __device__ uint64_t code_pitch() const { return (cols + kMxBlock - 1) / kMxBlock * 16; }
+  __host__ __device__ uint64_t blocks() const { return (cols + kMxBlock - 1) / kMxBlock; }
   __host__ __device__ uint64_t steps() const { return (cols + kMxStep - 1) / kMxStep; }
   __host__ __device__ uint64_t row_tiles() const { return (rows + kMxTileRows - 1) / kMxTileRows; }
+  // bytes of a row tile of one matrix, of all of them
+  __host__ __device__ uint64_t tile_bytes() const {
+    return blocks() * (kMxTileRows * 16) + steps() * (2 * kMxChunk);
+  }
+  __host__ __device__ uint64_t bytes() const { return matrices * row_tiles() * tile_bytes(); }
 };
+constexpr uint32_t kMxBlockBytes = kMxTileRows * 16;                    // a block of a tile
+constexpr uint32_t kMxStepBytes = 8 * kMxBlockBytes + 2 * kMxChunk;     // a full step of a tile
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) {
@@ -87,48 +97,83 @@ __device__ __forceinline__ float2 mx_decode2(uint32_t byte) {
 bool mx_shape(const char *who, uint64_t matrices, uint64_t rows, uint64_t cols);
 bool mx_dtype(const char *who, int dtype);
 
-// Offset of the scale of row r (in a tile whose scales take `chunks` chunks of 128 rows), block b of
-// the step.
+// Offset of the scale of row r (in a tile of up to 128 * chunks rows), block b of the step.
 __host__ __device__ __forceinline__ uint32_t mx_scale_offset(uint32_t r, uint32_t b, uint32_t chunks) {
   return ((b >> 2) * chunks + (r >> 7)) * kMxChunk + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (b & 3u);
 }
 
-// Eight consecutive elements of a row, of which `left` exist, as fp32 (the others 0).
-template <typename T, bool VEC>
-__device__ __forceinline__ void mx_load8(const T *src, int64_t left, float (&v)[8]) {
-  if (VEC) {
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (left > 0) raw = *reinterpret_cast<const uint4 *>(src);
-    const T *e = reinterpret_cast<const T *>(&raw);
+// The 32 elements of a block, of which `left` exist (the others are 0), as 16 words of two.
+// WIDE: 2 = the row is 32-byte aligned, 1 = 16-byte aligned, 0 = neither; left is a multiple of
+// 16, of 8, anything.
+template <int WIDE>
+__device__ __forceinline__ void mx_load_block(const void *src, int64_t left, uint32_t (&w)[16]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float<T>(e[i]);
+  for (int i = 0; i < 16; ++i) w[i] = 0;
+  if (WIDE == 2) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (left > 16 * h)
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[8 * h]), "=r"(w[8 * h + 1]), "=r"(w[8 * h + 2]), "=r"(w[8 * h + 3]),
+                       "=r"(w[8 * h + 4]), "=r"(w[8 * h + 5]), "=r"(w[8 * h + 6]), "=r"(w[8 * h + 7])
+                     : "l"((const uint8_t *)src + 32 * h));
+  } else if (WIDE == 1) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+      if (left > 8 * h) {
+        const uint4 v = __ldg((const uint4 *)src + h);
+        w[4 * h] = v.x;
+        w[4 * h + 1] = v.y;
+        w[4 * h + 2] = v.z;
+        w[4 * h + 3] = v.w;
+      }
   } else {
+    const uint16_t *e = (const uint16_t *)src;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_float<T>(src[i]) : 0.f;
+    for (int i = 0; i < 32; ++i)
+      if (i < left) w[i / 2] |= (uint32_t)__ldg(e + i) << (16 * (i & 1));
   }
 }
-
-// A warp quantises a step of a row: lane l holds elements 8 l .. 8 l + 7, four lanes a block.
-// Gives the lane's eight codes and the scale byte of its block.
-__device__ __forceinline__ void mx_quantize8(const float (&v)[8], uint32_t &codes, uint32_t &byte) {
+template <typename T>
+__device__ __forceinline__ float2 mx_unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 mx_unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ float2 mx_unpack2<__half>(uint32_t w) {
+  __half2 h;
+  memcpy(&h, &w, 4);
+  return __half22float2(h);
+}
+// Codes and scale byte of a block.
+template <typename T>
+__device__ __forceinline__ void mx_quantize_block(const uint32_t (&w)[16], uint32_t (&code)[4], uint32_t &byte) {
   uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, 1));
-  a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, 2));
+  for (int i = 0; i < 16; ++i) {
+    const float2 f = mx_unpack2<T>(w[i]);
+    a = max(a, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
+  }
   byte = mx_scale_byte(a);
   const float inv = mx_inverse_scale(byte);
-  codes = 0;
-  if (byte != 255u) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) codes |= mx_encode2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = mx_unpack2<T>(w[4 * i + j]);
+      c |= mx_encode2(f.x * inv, f.y * inv) << (8 * j);
+    }
+    code[i] = byte == 255u ? 0u : c;
   }
 }
-// The scale bytes of the half step that the lane's half warp holds, as the word at its address.
+// The scale bytes of the four blocks of 128 columns, which lanes l, l + 8, l + 16, l + 24 hold, as
+// the word at their address.
 __device__ __forceinline__ uint32_t mx_pack_scales(uint32_t byte, uint32_t lane) {
-  uint32_t word = byte << (8 * ((lane >> 2) & 3u));
-  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+  uint32_t word = byte << (8 * (lane >> 3));
   word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+  word |= __shfl_xor_sync(0xFFFFFFFFu, word, 16);
   return word;
 }
 

@@ -8,7 +8,7 @@
 //   quantise   turns the rows of x into codes and scales, in slot order, in the workspace
 //   product    one work item = (slot, tile of 128 rows of W, range of steps of 256 columns)
 // A tile of W is the M side of the MMA (128 tensor-memory lanes), a slot the N side (its columns).
-#include <cuda.h>
+#include <math.h>
 #include <string.h>
 
 #include <mutex>
@@ -21,8 +21,6 @@ namespace nz {
 
 constexpr uint32_t kMxMaxTok = 240;          // rows of x in a slot: what two accumulators leave room for
 constexpr uint32_t kMxMaxStages = 12;
-constexpr uint32_t kMxABytes = kMxTileRows * 128;            // codes of a tile's step
-constexpr uint32_t kMxSfABytes = 2 * kMxChunk;               // and its scales
 constexpr int kMxLinThreads = 192;           // TMA, MMA, 4 warps that store
 constexpr uint32_t kMxMaxExperts = 8192;
 constexpr uint32_t kMxNone = 0xFFFFFFFFu;
@@ -31,7 +29,8 @@ constexpr uint32_t kMxAcc1 = 256, kMxSfB = 240, kMxSfA = 496;
 
 struct MxLinearArgs {
   MxShape w;
-  const uint8_t *codes, *scales;
+  const uint8_t *packed;
+  uint64_t tile_bytes;
   const void *x;
   uint64_t x_stride;          // elements between rows of x
   uint32_t n_rows;            // rows of y
@@ -43,7 +42,8 @@ struct MxLinearArgs {
   // plan
   uint32_t tok, chunks;       // rows of a slot, 128-row chunks of its scales
   uint32_t slots;             // slots there can be
-  uint32_t row_tiles, steps;
+  uint32_t row_tiles, steps, blocks;
+  uint32_t x_step_bytes;      // a step of a slot: codes, scales
   uint32_t split;             // 1: the steps of a tile may be shared between CTAs
   uint32_t stages, stage_bytes;
   // workspace
@@ -52,8 +52,8 @@ struct MxLinearArgs {
   uint32_t *slot_expert, *slot_rows;       // stack: matrix of a slot, rows in it
   uint32_t *row_of;           // stack: row of y at every place of the slots
   uint32_t *place_of;         // stack: place of every row of y, kMxNone without a matrix
-  uint8_t *x_codes, *x_scales;
-  float *partial;             // split: two [tok][128] pieces a CTA
+  uint8_t *x_packed;
+  float *partial;             // split: a piece [tok][128] of every CTA
 };
 
 // ------------------------------------------------------------------ PTX
@@ -66,19 +66,12 @@ __device__ __forceinline__ void mx_fence_before() {
 __device__ __forceinline__ void mx_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-__device__ __forceinline__ void mx_tma_2d(uint32_t dst, const CUtensorMap *map, int32_t c0, int32_t c1,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-      "l"(map), "r"(bar), "r"(c0), "r"(c1)
-      : "memory");
-}
-// Shared-memory matrix descriptors: bits 0-13 address >> 4, 16-29 leading and 32-45 stride byte
-// offset >> 4, 46-47 version 1, 61-63 layout.  Codes: K-major, 128-byte swizzle (layout 2), groups
-// of 8 rows 1024 bytes apart.  Scales: no swizzle, groups of 8 rows of 16 bytes 128 bytes apart.
-__device__ __forceinline__ uint64_t mx_desc_codes(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// Shared-memory matrix descriptors, no swizzle: bits 0-13 address >> 4, 16-29 leading and 32-45
+// stride byte offset >> 4, 46-47 version 1.  Codes of a tile of `rows` rows, K-major: groups of 8
+// rows of 16 bytes are 128 bytes apart (stride), the next 16 bytes of a row 16 * rows (leading).
+// Scales: groups of 8 rows of 16 bytes 128 bytes apart, one column of 16 bytes.
+__device__ __forceinline__ uint64_t mx_desc_codes(uint32_t addr, uint32_t rows) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)rows << 16) | (8ull << 32) | (1ull << 46);
 }
 __device__ __forceinline__ uint64_t mx_desc_scales(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | (8ull << 32) | (1ull << 46);
@@ -122,6 +115,23 @@ __device__ __forceinline__ bool mx_wait(uint32_t bar, uint32_t parity, const vol
     if ((it & 63u) == 63u && *abort_flag) return false;
   }
   return false;
+}
+// The same for a converged warp: one verdict for all lanes.
+__device__ __forceinline__ bool mx_wait_warp(uint32_t bar, uint32_t parity, const volatile uint32_t *abort_flag) {
+  return __all_sync(0xFFFFFFFFu, mx_wait(bar, parity, abort_flag));
+}
+// One lane of a converged warp.  The instructions below take their operands from the registers that
+// a warp shares; a branch that the compiler knows to be one lane's leaves the operands there, while
+// under `lane == 0` every one is moved across first (a step of four products took 1000 cycles to
+// issue that way).
+__device__ __forceinline__ bool mx_elect() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
 // Barrier of the four warps that store, and a vote over them: the same verdict for all, so that none
 // waits here for one that has left.
@@ -217,104 +227,102 @@ __global__ void __launch_bounds__(kMxRouteThreads) mx4_route_kernel(const MxLine
 }
 
 // ------------------------------------------------------------------ the rows of x
-// One warp per (row of x, step): quantised once, written to the place of every row of y it serves.
-// Rows of y without a matrix are set to zero here.
-template <typename T, bool VEC>
+// As in mx4_quantize_kernel a thread takes a block, a warp eight rows of x of four blocks.  A row is
+// quantised once and written to the place of every row of y it serves.  Rows of y without a matrix
+// are set to zero here.
+template <typename T, int WIDE>
 __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearArgs p) {
   if (p.experts) dependent_wait();
   dependent_trigger();
   const uint32_t lane = threadIdx.x & 31;
-  const uint32_t pitch = (uint32_t)p.w.code_pitch(), cols = (uint32_t)p.w.cols;
   if (p.split && !p.experts)
     for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < p.slots * p.row_tiles; i += gridDim.x * 256)
       p.counters[i] = 0;
-  const uint64_t total = (uint64_t)(p.n_rows / p.per_input) * p.steps;
+  const uint32_t halves = 2 * p.steps, inputs = p.n_rows / p.per_input;
+  const uint64_t total = (uint64_t)((inputs + 7) / 8) * halves;
   for (uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (uint64_t)gridDim.x * 8) {
-    const uint32_t row = (uint32_t)(w / p.steps), step = (uint32_t)(w - (uint64_t)row * p.steps);
-    const uint32_t col = step * kMxStep + lane * 8;
-    float v[8];
-    mx_load8<T, VEC>((const T *)p.x + row * p.x_stride + col, (int64_t)cols - col, v);
-    uint32_t code, byte;
-    mx_quantize8(v, code, byte);
+    const uint32_t group = (uint32_t)(w / halves), half = (uint32_t)(w - (uint64_t)group * halves);
+    const uint32_t row = group * 8 + (lane & 7u), block = half * 4 + (lane >> 3);
+    uint32_t v[16], code[4], byte;
+    const int64_t left = row < inputs ? (int64_t)p.w.cols - (int64_t)block * kMxBlock : 0;
+    mx_load_block<WIDE>((const T *)p.x + row * p.x_stride + (uint64_t)block * kMxBlock, left, v);
+    mx_quantize_block<T>(v, code, byte);
     const uint32_t word = mx_pack_scales(byte, lane);
+    if (row >= inputs) continue;
     for (uint32_t j = 0; j < p.per_input; ++j) {
       const uint32_t r = row * p.per_input + j;
       const uint32_t place = p.experts ? p.place_of[r] : r;
       if (place == kMxNone) {
-        const uint64_t n = p.w.rows, a = n * step / p.steps, b = n * (step + 1) / p.steps;
-        for (uint64_t i = a + lane; i < b; i += 32) ((T *)p.y)[r * n + i] = from_float<T>(0.f);
+        // the row's lanes of all its warps share it out
+        const uint64_t n = p.w.rows;
+        for (uint64_t i = block; i < n; i += 4 * halves) ((T *)p.y)[r * n + i] = from_float<T>(0.f);
         continue;
       }
-      if (col < 2 * pitch) *reinterpret_cast<uint32_t *>(p.x_codes + (uint64_t)place * pitch + col / 2) = code;
-      if ((lane & 15u) == 0) {
-        const uint32_t slot = place / p.tok, i = place - slot * p.tok;
-        *reinterpret_cast<uint32_t *>(p.x_scales +
-                                      ((uint64_t)slot * p.steps + step) * (2 * kMxChunk * p.chunks) +
-                                      mx_scale_offset(i, lane >> 2, p.chunks)) = word;
-      }
+      const uint32_t slot = place / p.tok, i = place - slot * p.tok;
+      uint8_t *step = p.x_packed + ((uint64_t)slot * p.steps + (half >> 1)) * p.x_step_bytes;
+      *reinterpret_cast<uint4 *>(step + ((block & 7u) * p.tok + i) * 16) =
+          make_uint4(code[0], code[1], code[2], code[3]);
+      if (lane < 8)
+        *reinterpret_cast<uint32_t *>(step + 128 * p.tok + mx_scale_offset(i, (half & 1) * 4, p.chunks)) = word;
     }
   }
 }
 
 // ------------------------------------------------------------------ the product
-// The items of a CTA, in the same order for every role of it.  Without splitting a CTA takes every
-// gridDim.x-th tile; with it, an equal share of all steps of all tiles, one after the other, so
-// that at most its first and its last tile are shared with its neighbours.
+// The items of a CTA, in the same order for every role of it.  Where there are at least two CTAs
+// for every tile, its steps are divided among `pieces` of them; else a CTA takes every
+// gridDim.x-th tile.  What an item needs from the slot tables is fetched an item ahead.
+struct MxItem {
+  uint32_t slot, row_tile, tile, piece, k0, k1, expert, rows;
+};
 struct MxItems {
-  uint32_t tiles, steps, split, row_tiles, n_slots;
-  uint32_t tile;              // next tile
-  uint64_t unit, end;         // split: next and last step
-  uint32_t slot, row_tile, k0, k1;     // current item
+  const MxLinearArgs &p;
+  uint32_t n_slots, tiles, pieces;
+  uint32_t at;                // number of the item that is fetched
+  MxItem ahead;
 
-  __device__ __forceinline__ MxItems(const MxLinearArgs &p, uint32_t n_slots_)
-      : tiles(n_slots_ * p.row_tiles), steps(p.steps), split(p.split), row_tiles(p.row_tiles),
-        n_slots(n_slots_), tile(blockIdx.x), unit(0), end(0), slot(0), row_tile(0), k0(0), k1(0) {
-    if (split) {
-      const uint64_t units = (uint64_t)tiles * steps, ctas = sharers(units);
-      if (blockIdx.x < ctas) {
-        unit = units * blockIdx.x / ctas;
-        end = units * (blockIdx.x + 1) / ctas;
-      }
+  __device__ __forceinline__ MxItems(const MxLinearArgs &p_, uint32_t n_slots_)
+      : p(p_), n_slots(n_slots_), tiles(n_slots_ * p_.row_tiles), pieces(1), at(blockIdx.x) {
+    if (p.split && tiles) {
+      const uint32_t most = gridDim.x / tiles;
+      pieces = most < 1 ? 1 : most < p.steps ? most : p.steps;
     }
-  }
-  // CTAs with a share: every share has a step at least
-  __device__ __forceinline__ uint64_t sharers(uint64_t units) const {
-    return units < gridDim.x ? units : gridDim.x;
-  }
-  // the CTA whose share has this step
-  __device__ __forceinline__ uint32_t owner(uint64_t at) const {
-    const uint64_t units = (uint64_t)tiles * steps;
-    return (uint32_t)(((at + 1) * sharers(units) - 1) / units);
+    fetch();
   }
   // Neighbouring tiles share a tile of W with up to 8 slots, and those slots with the next tiles
   // of W, so that what runs at a time reads little from outside L2.
-  __device__ __forceinline__ void place(uint32_t t) {
-    const uint32_t band = t / (8 * row_tiles), rest = t - band * 8 * row_tiles;
+  __device__ __forceinline__ void fetch() {
+    if (at >= tiles * pieces) return;
+    const uint32_t t = at / pieces;
+    ahead.tile = t;
+    ahead.piece = at - t * pieces;
+    ahead.k0 = p.steps * ahead.piece / pieces;
+    ahead.k1 = p.steps * (ahead.piece + 1) / pieces;
+    const uint32_t band = t / (8 * p.row_tiles), rest = t - band * 8 * p.row_tiles;
     const uint32_t wide = n_slots - band * 8 < 8 ? n_slots - band * 8 : 8;
-    row_tile = rest / wide;
-    slot = band * 8 + rest - row_tile * wide;
-  }
-  __device__ __forceinline__ bool next() {
-    if (split) {
-      if (unit >= end) return false;
-      tile = (uint32_t)(unit / steps);
-      k0 = (uint32_t)(unit - (uint64_t)tile * steps);
-      const uint64_t left = end - unit;
-      k1 = left < steps - k0 ? k0 + (uint32_t)left : steps;
-      unit += k1 - k0;
-      place(tile);
-      return true;
+    ahead.row_tile = rest / wide;
+    ahead.slot = band * 8 + rest - ahead.row_tile * wide;
+    if (p.experts) {
+      ahead.expert = __ldcg(p.slot_expert + ahead.slot);
+      ahead.rows = __ldcg(p.slot_rows + ahead.slot);
+    } else {
+      ahead.expert = 0;
+      ahead.rows = min(p.tok, p.n_rows - ahead.slot * p.tok);
     }
-    if (tile >= tiles) return false;
-    k0 = 0;
-    k1 = steps;
-    place(tile);
-    tile += gridDim.x;
+  }
+  __device__ __forceinline__ bool next(MxItem &item) {
+    if (at >= tiles * pieces) return false;
+    item = ahead;
+    // the same in all lanes; the shuffle lets the compiler know
+    item.expert = __shfl_sync(0xFFFFFFFFu, item.expert, 0);
+    item.rows = __shfl_sync(0xFFFFFFFFu, item.rows, 0);
+    at += gridDim.x;
+    fetch();
     return true;
   }
 };
 
-// Shared-memory map: stages (1024-aligned; codes of W, codes of x, scales of W, scales of x), then
+// Shared-memory map: stages (a step of a tile of W, a step of a slot), then
 constexpr uint32_t kMxBarFull = 0, kMxBarEmpty = 8 * kMxMaxStages, kMxBarAccFull = 16 * kMxMaxStages,
                    kMxBarAccEmpty = kMxBarAccFull + 16, kMxBarDrain = kMxBarAccEmpty + 16,
                    kMxTmemSlot = kMxBarDrain + 8,
@@ -323,16 +331,14 @@ static_assert(kMxLastSlot + 4 <= kMxMiscBytes, "barriers");
 
 template <typename T>
 __global__ void __launch_bounds__(kMxLinThreads, 1)
-mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ CUtensorMap w_map,
-                   const __grid_constant__ CUtensorMap x_map) {
+mx4_product_kernel(const MxLinearArgs p) {
   extern __shared__ uint8_t mx_smem[];
-  const uint32_t base = (smem_u32(mx_smem) + 1023u) & ~1023u;
+  const uint32_t base = (smem_u32(mx_smem) + 127u) & ~127u;
   const uint32_t misc_a = base + p.stages * p.stage_bytes;
   uint8_t *misc = mx_smem + (misc_a - smem_u32(mx_smem));
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(misc + kMxAbortSlot);
   volatile uint32_t *last_flag = reinterpret_cast<volatile uint32_t *>(misc + kMxLastSlot);
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t x_bytes = p.tok * 128, sfb_bytes = p.chunks * 2 * kMxChunk;
+  const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -359,125 +365,131 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ CUtensorMap w_m
   mx_fence_before();
   __syncthreads();
   mx_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(misc + kMxTmemSlot);
-  const uint32_t n_slots = p.experts ? *p.n_slots : p.slots;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t *>(misc + kMxTmemSlot), 0);
+  const uint32_t n_slots = p.experts ? __shfl_sync(0xFFFFFFFFu, __ldcg(p.n_slots), 0) : p.slots;
   MxItems items(p, n_slots);
 
   if (warp == 0) {
     // ---------------------------------------------------------------- copies
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0;
-      uint64_t done = 0;
-      bool ok = true;
-      while (ok && items.next()) {
-        const uint32_t e = p.experts ? p.slot_expert[items.slot] : 0;
-        const int32_t w_row = (int32_t)((uint64_t)e * p.w.rows + items.row_tile * kMxTileRows);
-        const uint8_t *sfa = p.scales + ((uint64_t)e * p.row_tiles + items.row_tile) * p.steps * kMxSfABytes;
-        const uint8_t *sfb = p.x_scales + (uint64_t)items.slot * p.steps * sfb_bytes;
-        for (uint32_t k = items.k0; k < items.k1; ++k, ++done) {
-          if (done >= p.stages && !mx_wait(misc_a + kMxBarEmpty + 8 * stage, phase ^ 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const uint32_t at = base + stage * p.stage_bytes, bar = misc_a + kMxBarFull + 8 * stage;
-          mbar_expect_tx(bar, p.stage_bytes);
-          mx_tma_2d(at, &w_map, (int32_t)(k * 128), w_row, bar);
-          mx_tma_2d(at + kMxABytes, &x_map, (int32_t)(k * 128), (int32_t)(items.slot * p.tok), bar);
-          bulk_g2s(at + kMxABytes + x_bytes, sfa + (uint64_t)k * kMxSfABytes, kMxSfABytes, bar);
-          bulk_g2s(at + kMxABytes + x_bytes + kMxSfABytes, sfb + (uint64_t)k * sfb_bytes, sfb_bytes, bar);
-          if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1;
-          }
+    uint32_t stage = 0, phase = 0;
+    uint64_t done = 0;
+    bool ok = true;
+    MxItem it;
+    while (ok && items.next(it)) {
+      const uint8_t *w = p.packed + ((uint64_t)it.expert * p.row_tiles + it.row_tile) * p.tile_bytes;
+      const uint8_t *x = p.x_packed + (uint64_t)it.slot * p.steps * p.x_step_bytes;
+      for (uint32_t k = it.k0; k < it.k1; ++k, ++done) {
+        if (done >= p.stages && !mx_wait_warp(misc_a + kMxBarEmpty + 8 * stage, phase ^ 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        const uint32_t at = base + stage * p.stage_bytes, bar = misc_a + kMxBarFull + 8 * stage;
+        const uint32_t w_bytes = min(8u, p.blocks - 8 * k) * kMxBlockBytes + 2 * kMxChunk;
+        if (mx_elect()) {
+          mbar_expect_tx(bar, w_bytes + p.x_step_bytes);
+          bulk_g2s(at, w + (uint64_t)k * kMxStepBytes, w_bytes, bar);
+          bulk_g2s(at + kMxStepBytes, x + (uint64_t)k * p.x_step_bytes, p.x_step_bytes, bar);
+        }
+        __syncwarp();
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-      if (!ok) {
-        if (p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
-        *abort_flag = 1;
-      }
+    }
+    if (!ok) {
+      if (lane == 0 && p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
+      *abort_flag = 1;
       // copies still in flight land before the CTA's shared memory is given away: after an abort
       // nobody else waits for them
-      if (!ok) {
-        const uint64_t from = done > p.stages ? done - p.stages : 0;
-        for (uint64_t i = from; i < done; ++i) {
-          const uint32_t s = (uint32_t)(i % p.stages), ph = (uint32_t)(i / p.stages) & 1u;
-          for (uint32_t it = 0; it < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarFull + 8 * s, ph); ++it) {
-          }
+      for (uint64_t i = done > p.stages ? done - p.stages : 0; i < done; ++i) {
+        const uint32_t s = (uint32_t)(i % p.stages), ph = (uint32_t)(i / p.stages) & 1u;
+        for (uint32_t n = 0; n < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarFull + 8 * s, ph); ++n) {
         }
       }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- tensor cores
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0, item = 0;
-      bool ok = true;
-      const uint32_t k64 = (uint32_t)((p.w.cols + 63) / 64);
-      while (ok && items.next()) {
-        const uint32_t rows = p.experts ? p.slot_rows[items.slot]
-                                        : min(p.tok, p.n_rows - items.slot * p.tok);
-        const uint32_t n = (rows + 15u) & ~15u;
-        // 4-bit operands (type 1), e8m0 scales, M = 128
-        const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | (1u << 27);
-        const uint32_t acc = item & 1u, d = tmem + (acc ? kMxAcc1 : 0u);
-        if (item >= 2 && !mx_wait(misc_a + kMxBarAccEmpty + 8 * acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) {
+    uint32_t stage = 0, phase = 0, item = 0;
+    bool ok = true;
+    const uint32_t k64 = (p.blocks + 1) / 2;
+    MxItem it;
+    while (ok && items.next(it)) {
+      const uint32_t n = (it.rows + 15u) & ~15u;
+      // 4-bit operands (type 1), e8m0 scales, M = 128
+      const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | (1u << 27);
+      const uint32_t acc = item & 1u, d = tmem + (acc ? kMxAcc1 : 0u);
+      if (item >= 2 && !mx_wait_warp(misc_a + kMxBarAccEmpty + 8 * acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) {
+        ok = false;
+        break;
+      }
+      mx_fence_after();
+      for (uint32_t k = it.k0; k < it.k1; ++k) {
+        if (!mx_wait_warp(misc_a + kMxBarFull + 8 * stage, phase, abort_flag)) {
           ok = false;
           break;
         }
         mx_fence_after();
-        for (uint32_t k = items.k0; k < items.k1; ++k) {
-          if (!mx_wait(misc_a + kMxBarFull + 8 * stage, phase, abort_flag)) {
-            ok = false;
-            break;
-          }
-          mx_fence_after();
-          const uint32_t at = base + stage * p.stage_bytes;
-          const uint64_t ad = mx_desc_codes(at), bd = mx_desc_codes(at + kMxABytes);
-          const uint32_t sfa = at + kMxABytes + x_bytes, sfb = sfa + kMxSfABytes;
+        const uint32_t at = base + stage * p.stage_bytes;
+        const uint64_t ad = mx_desc_codes(at, kMxTileRows), bd = mx_desc_codes(at + kMxStepBytes, p.tok);
+        const uint64_t sfa = mx_desc_scales(at + min(8u, p.blocks - 8 * k) * kMxBlockBytes);
+        const uint64_t sfb = mx_desc_scales(at + kMxStepBytes + 128 * p.tok);
+        const uint32_t last = min(4u, k64 - 4 * k);
+        if (mx_elect()) {
           // copies and products of one thread run in order: the scales of the step before have
           // been used when these replace them
 #pragma unroll
           for (uint32_t h = 0; h < 2; ++h) {
-            mx_copy_scales(tmem + kMxSfA + 4 * h, mx_desc_scales(sfa + h * kMxChunk));
-            for (uint32_t c = 0; c < p.chunks; ++c)
-              mx_copy_scales(tmem + kMxSfB + 8 * h + 4 * c, mx_desc_scales(sfb + (h * p.chunks + c) * kMxChunk));
+            mx_copy_scales(tmem + kMxSfA + 4 * h, sfa + h * (kMxChunk >> 4));
+            mx_copy_scales(tmem + kMxSfB + 8 * h, sfb + h * p.chunks * (kMxChunk >> 4));
+            if (p.chunks == 2) mx_copy_scales(tmem + kMxSfB + 8 * h + 4, sfb + (2 * h + 1) * (kMxChunk >> 4));
           }
-          const uint32_t last = min(4u, k64 - 4 * k);
-          for (uint32_t j = 0; j < last; ++j) {
-            // 64 columns are 32 bytes; the scales of two of them share a tensor-memory column, the
-            // second starts at byte 2
-            const uint32_t id = (j & 1u) * 2u;
-            mx_mma(d, ad + 2 * j, bd + 2 * j, idesc0 | (id << 4) | (id << 29), tmem + kMxSfA + 4 * (j >> 1),
-                   tmem + kMxSfB + 8 * (j >> 1), (k > items.k0) | (j > 0));
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) {
+            // 64 columns are two blocks; the scales of four share a tensor-memory column, the second
+            // product's start at byte 2
+            constexpr uint32_t kSecond = (2u << 4) | (2u << 29);
+            if (j < last)
+              mx_mma(d, ad + 2 * j * kMxTileRows, bd + 2 * j * p.tok, idesc0 | ((j & 1u) ? kSecond : 0u),
+                     tmem + kMxSfA + 4 * (j >> 1), tmem + kMxSfB + 8 * (j >> 1), (k > it.k0) | (j > 0));
           }
           mx_commit(misc_a + kMxBarEmpty + 8 * stage);
-          if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          if (k + 1 == it.k1) mx_commit(misc_a + kMxBarAccFull + 8 * acc);
         }
-        if (ok) mx_commit(misc_a + kMxBarAccFull + 8 * acc);
-        ++item;
+        __syncwarp();
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      if (!ok) {
-        if (p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
-        *abort_flag = 1;
-        // what has been issued still uses shared and tensor memory
-        mx_commit(misc_a + kMxBarDrain);
-        for (uint32_t it = 0; it < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarDrain, 0); ++it) {
-        }
+      ++item;
+    }
+    if (!ok) {
+      if (lane == 0 && p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
+      *abort_flag = 1;
+      // what has been issued still uses shared and tensor memory
+      if (mx_elect()) mx_commit(misc_a + kMxBarDrain);
+      __syncwarp();
+      for (uint32_t n = 0; n < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarDrain, 0); ++n) {
       }
     }
   } else {
     // ---------------------------------------------------------------- results
     const uint32_t sub = warp & 3u;                   // tensor-memory lanes 32 sub .. + 31
     uint32_t item = 0;
-    while (items.next()) {
-      const uint32_t rows = p.experts ? p.slot_rows[items.slot]
-                                      : min(p.tok, p.n_rows - items.slot * p.tok);
-      const uint32_t e = p.experts ? p.slot_expert[items.slot] : 0;
-      const uint32_t feature = items.row_tile * kMxTileRows + 32 * sub + lane;
+    MxItem it;
+    while (items.next(it)) {
+      const uint32_t rows = it.rows, place0 = it.slot * p.tok;
+      const uint32_t feature = it.row_tile * kMxTileRows + 32 * sub + lane;
       const bool real = feature < p.w.rows;
-      const float bias = p.bias && real ? to_float<T>(((const T *)p.bias)[e * p.w.rows + feature]) : 0.f;
+      const float bias = p.bias && real ? to_float<T>(((const T *)p.bias)[it.expert * p.w.rows + feature]) : 0.f;
+      T *y = (T *)p.y + feature;
+      // lane i of 16 knows the row of y of column c0 + i; fetched 16 columns ahead
+      auto row_at = [&](uint32_t c) -> uint32_t {
+        if (!p.experts) return place0 + c + (lane & 15u);
+        return c + (lane & 15u) < rows ? p.row_of[place0 + c + (lane & 15u)] : 0u;
+      };
+      uint32_t row_next = row_at(0);
       const uint32_t acc = item & 1u, d = tmem + (acc ? kMxAcc1 : 0u) + ((32u * sub) << 16);
       if (!mx_store_all(mx_wait(misc_a + kMxBarAccFull + 8 * acc, (item >> 1) & 1u, abort_flag))) {
         if (lane == 0 && p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
@@ -485,14 +497,13 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ CUtensorMap w_m
         break;
       }
       mx_fence_after();
-      const uint32_t whole = items.k0 == 0 && items.k1 == items.steps;
-      const uint32_t place0 = items.slot * p.tok;
-      float *piece = whole ? nullptr
-                           : p.partial + ((uint64_t)blockIdx.x * 2 + (items.k0 == 0)) * p.tok * kMxTileRows +
-                                 32 * sub + lane;
+      const bool whole = items.pieces == 1;
+      float *piece = whole ? nullptr : p.partial + (uint64_t)blockIdx.x * p.tok * kMxTileRows + 32 * sub + lane;
       for (uint32_t c0 = 0; c0 < rows; c0 += 16) {
         uint32_t v[16];
         mx_tmem_ld16(d + c0, v);
+        const uint32_t row_here = row_next;
+        row_next = row_at(c0 + 16);
         mx_tmem_ld_wait();
         if (c0 + 16 >= rows) {
           // the last columns are out: the tensor cores may have this accumulator again
@@ -505,47 +516,46 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ CUtensorMap w_m
           if (c0 + i >= rows) break;
           if (!whole) {
             piece[(uint64_t)(c0 + i) * kMxTileRows] = __uint_as_float(v[i]);
-          } else if (real) {
-            const uint64_t r = p.experts ? p.row_of[place0 + c0 + i] : place0 + c0 + i;
-            ((T *)p.y)[r * p.w.rows + feature] = from_float<T>(__uint_as_float(v[i]) + bias);
+          } else {
+            const uint64_t r = __shfl_sync(0xFFFFFFFFu, row_here, i);
+            if (real) y[r * p.w.rows] = from_float<T>(__uint_as_float(v[i]) + bias);
           }
         }
       }
       if (!whole) {
         // The CTA that brings the last piece of a tile adds all of them, in the order of the steps.
-        const uint32_t t = (uint32_t)((items.unit - 1) / items.steps);
-        const uint32_t first = items.owner((uint64_t)t * items.steps);
-        const uint32_t last = items.owner((uint64_t)(t + 1) * items.steps - 1);
         __threadfence();
         mx_store_barrier();
         if (threadIdx.x == 64) {
-          const uint32_t seen = atomicAdd(p.counters + t, 1u);
+          const uint32_t seen = atomicAdd(p.counters + it.tile, 1u);
           __threadfence();
-          *last_flag = seen == last - first;
+          *last_flag = seen == items.pieces - 1;
         }
         mx_store_barrier();
-        const bool mine = *last_flag != 0;
-        mx_store_barrier();                           // the flag may be written again
-        if (mine && real) {
-          __threadfence();
-          constexpr uint32_t kBatch = 8;
-          for (uint32_t t0 = 0; t0 < rows; t0 += kBatch) {
-            float sum[kBatch] = {};
-            for (uint32_t c = first; c <= last; ++c) {
-              const float *from = p.partial + ((uint64_t)c * 2 + (c == first)) * p.tok * kMxTileRows +
-                                  32 * sub + lane;
-              float add[kBatch];
+        if (*last_flag) {
+          const float *from = p.partial + (uint64_t)it.tile * items.pieces * p.tok * kMxTileRows + 32 * sub + lane;
+          constexpr uint32_t kCols = 8, kPieces = 4;      // loads in flight
+          for (uint32_t c0 = 0; c0 < rows; c0 += kCols) {
+            float sum[kCols] = {};
+            const uint32_t row_here = row_at(c0 & ~15u);
+            for (uint32_t q0 = 0; q0 < items.pieces; q0 += kPieces) {
+              float add[kPieces][kCols];
 #pragma unroll
-              for (uint32_t i = 0; i < kBatch; ++i)
-                add[i] = t0 + i < rows ? __ldcg(from + (uint64_t)(t0 + i) * kMxTileRows) : 0.f;
+              for (uint32_t q = 0; q < kPieces; ++q)
 #pragma unroll
-              for (uint32_t i = 0; i < kBatch; ++i) sum[i] += add[i];
+                for (uint32_t i = 0; i < kCols; ++i)
+                  add[q][i] = q0 + q < items.pieces && c0 + i < rows
+                                  ? __ldcg(from + ((uint64_t)(q0 + q) * p.tok + c0 + i) * kMxTileRows) : 0.f;
+#pragma unroll
+              for (uint32_t q = 0; q < kPieces; ++q)
+#pragma unroll
+                for (uint32_t i = 0; i < kCols; ++i) sum[i] += add[q][i];
             }
 #pragma unroll
-            for (uint32_t i = 0; i < kBatch; ++i) {
-              if (t0 + i >= rows) break;
-              const uint64_t r = p.experts ? p.row_of[place0 + t0 + i] : place0 + t0 + i;
-              ((T *)p.y)[r * p.w.rows + feature] = from_float<T>(sum[i] + bias);
+            for (uint32_t i = 0; i < kCols; ++i) {
+              if (c0 + i >= rows) break;
+              const uint64_t r = __shfl_sync(0xFFFFFFFFu, row_here, (c0 & 15u) + i);
+              if (real) y[r * p.w.rows] = from_float<T>(sum[i] + bias);
             }
           }
         }
@@ -565,59 +575,61 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ CUtensorMap w_m
 }
 
 // --------------------------------------------------------------------- host
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn mx_encode_tiled() {
-  static std::once_flag once;
-  static EncodeTiledFn fn = nullptr;
-  std::call_once(once, [] {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = (EncodeTiledFn)ptr;
-  });
-  return fn;
-}
-// Codes as a matrix of bytes [rows, pitch], fetched 128 columns of bytes by `box` rows at a time.
-static bool mx_map(CUtensorMap *map, const void *codes, uint64_t rows, uint64_t pitch, uint32_t box) {
-  const cuuint64_t dim[2] = {pitch, rows};
-  const cuuint64_t stride[1] = {pitch};
-  const cuuint32_t size[2] = {128, box}, step[2] = {1, 1};
-  return mx_encode_tiled()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dim, stride,
-                           size, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 struct MxPlan {
-  uint32_t tok, chunks, row_tiles, steps, split, grid, stages, stage_bytes;
+  uint32_t tok, chunks, row_tiles, steps, split, grid, stages, stage_bytes, x_step_bytes;
   uint64_t slots;
-  uint64_t counters, slot_expert, slot_rows, row_of, place_of, x_codes, x_scales, partial, bytes;
+  uint64_t counters, slot_expert, slot_rows, row_of, place_of, x_packed, partial, bytes;
 };
+
+// The rows of a slot, by an estimate of the time (in cycles) that the product takes with them: an
+// SM takes in about 40 bytes a cycle, the tensor cores need 2 cycles a row and step, and what
+// an item costs beside its steps grows with its rows.
+static double mx_cost(uint64_t tok, double slots, uint64_t row_tiles, uint64_t steps, uint32_t sms) {
+  const double tiles = slots * (double)row_tiles;
+  double pieces = 1, waves = ceil(tiles / sms);
+  if (tiles * 2 <= sms) {
+    pieces = floor(sms / tiles);
+    if (pieces > (double)steps) pieces = (double)steps;
+    waves = 1;
+  }
+  const double load = (kMxStepBytes + tok * 128.0 + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 40.0;
+  const double mma = 2.0 * tok;
+  const double step = load > mma ? load : mma;
+  return waves * (ceil(steps / pieces) * step + 1000 + 8.0 * tok) +
+         (pieces > 1 ? 2000 + 4.0 * tok * pieces : 0);
+}
 
 static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) {
   const uint32_t sms = (uint32_t)sm_count();
   g.row_tiles = (uint32_t)w.row_tiles();
   g.steps = (uint32_t)w.steps();
   const uint64_t groups = grouped ? (w.matrices < n_rows ? w.matrices : n_rows) : 1;
-  const uint64_t average = (n_rows + groups - 1) / groups;
-  uint64_t tok = (average + 15) / 16 * 16;
-  if (tok > kMxMaxTok) tok = kMxMaxTok;
+  // matrices that are likely to be named, and half a slot of each that stays empty
+  const double hit = grouped ? (double)w.matrices * (1 - pow(1 - 1.0 / (double)w.matrices, (double)n_rows)) : 1;
+  uint64_t tok = 16;
+  double best = 0;
+  for (uint64_t t = 16; t <= kMxMaxTok; t += 16) {
+    double slots = grouped ? (double)n_rows / t + hit / 2 : ceil((double)n_rows / t);
+    if (slots < hit) slots = hit;
+    const double cost = mx_cost(t, slots, g.row_tiles, g.steps, sms);
+    if (t == 16 || cost < best) {
+      best = cost;
+      tok = t;
+    }
+  }
   g.tok = (uint32_t)tok;
   g.chunks = g.tok > 128 ? 2 : 1;
   // every matrix's last slot may be short
   g.slots = grouped ? (n_rows - groups) / tok + groups : (n_rows + tok - 1) / tok;
   const uint64_t tiles = g.slots * g.row_tiles;
   if (g.slots * tok >= (1ull << 31) || tiles >= (1ull << 31)) return false;
-  g.split = tiles < 4ull * sms;
+  // a stack may turn out to need fewer tiles than there can be
+  g.split = g.steps > 1 && (grouped ? tiles < 2ull * sms : 2 * tiles <= sms);
   const uint64_t units = g.split ? tiles * g.steps : tiles;
   g.grid = (uint32_t)(units < sms ? units : sms);
-  g.stage_bytes = kMxABytes + g.tok * 128 + kMxSfABytes + g.chunks * 2 * kMxChunk;
-  g.stages = (kMaxDynamicSmem - 1024 - kMxMiscBytes) / g.stage_bytes;
+  g.x_step_bytes = g.tok * 128 + g.chunks * 2 * kMxChunk;
+  g.stage_bytes = kMxStepBytes + g.x_step_bytes;
+  g.stages = (kMaxDynamicSmem - 128 - kMxMiscBytes) / g.stage_bytes;
   if (g.stages > kMxMaxStages) g.stages = kMxMaxStages;
   uint64_t at = 256;
   auto take = [&](uint64_t bytes) {
@@ -630,9 +642,8 @@ static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) 
   g.slot_rows = take(grouped ? g.slots * 4 : 0);
   g.row_of = take(grouped ? g.slots * tok * 4 : 0);
   g.place_of = take(grouped ? n_rows * 4 : 0);
-  g.x_codes = take(g.slots * tok * w.code_pitch());
-  g.x_scales = take(g.slots * g.steps * g.chunks * 2 * kMxChunk);
-  g.partial = take(g.split ? (uint64_t)g.grid * 2 * tok * kMxTileRows * 4 : 0);
+  g.x_packed = take(g.slots * g.steps * g.x_step_bytes);
+  g.partial = take(g.split ? (uint64_t)g.grid * tok * kMxTileRows * 4 : 0);
   g.bytes = at;
   return true;
 }
@@ -652,15 +663,16 @@ static cudaError_t mx_opt_in(K kern, int bytes, bool (&done)[kMaxDeviceOrdinals]
 }
 
 template <typename T>
-static int mx_launch(const MxLinearArgs &p, const MxPlan &g, const CUtensorMap &w_map,
-                     const CUtensorMap &x_map, cudaStream_t st) {
+static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
   static bool product_done[kMaxDeviceOrdinals] = {}, route_done[kMaxDeviceOrdinals] = {};
   NZ_CUDA_TRY(mx_opt_in(mx4_product_kernel<T>, (int)kMaxDynamicSmem, product_done));
-  const bool vec = p.w.cols % 8 == 0 && p.x_stride % 8 == 0 && ((uintptr_t)p.x & 15) == 0;
-  const uint64_t warps = (uint64_t)(p.n_rows / p.per_input) * p.steps, blocks = (warps + 7) / 8;
+  const uintptr_t apart = (uintptr_t)p.x | (uintptr_t)(p.x_stride * 2) | (uintptr_t)(p.w.cols * 2);
+  const uint64_t warps = (uint64_t)((p.n_rows / p.per_input + 7) / 8) * 2 * p.steps, blocks = (warps + 7) / 8;
   const unsigned most = (unsigned)sm_count() * 8;
   const unsigned grid = blocks < most ? (unsigned)blocks : most;
-  auto rows_kernel = vec ? mx4_quantize_rows_kernel<T, true> : mx4_quantize_rows_kernel<T, false>;
+  auto rows_kernel = apart % 32 == 0   ? mx4_quantize_rows_kernel<T, 2>
+                     : apart % 16 == 0 ? mx4_quantize_rows_kernel<T, 1>
+                                       : mx4_quantize_rows_kernel<T, 0>;
   if (p.experts) {
     NZ_CUDA_TRY(mx_opt_in(mx4_route_kernel, (int)(kMxMaxExperts * 8), route_done));
     mx4_route_kernel<<<1, kMxRouteThreads, p.w.matrices * 8, st>>>(p);
@@ -670,8 +682,8 @@ static int mx_launch(const MxLinearArgs &p, const MxPlan &g, const CUtensorMap &
     rows_kernel<<<grid, 256, 0, st>>>(p);
     NZ_LAUNCH_CHECK("mx4_quantize_rows_kernel");
   }
-  const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + kMxMiscBytes;
-  NZ_CUDA_TRY(launch_dependent(mx4_product_kernel<T>, g.grid, kMxLinThreads, smem, st, p, w_map, x_map));
+  const size_t smem = 128 + (size_t)p.stages * p.stage_bytes + kMxMiscBytes;
+  NZ_CUDA_TRY(launch_dependent(mx4_product_kernel<T>, g.grid, kMxLinThreads, smem, st, p));
   return NZ_OK;
 }
 
@@ -689,11 +701,10 @@ extern "C" uint64_t nz_mx4_linear_workspace_bytes(uint64_t matrices, uint64_t ro
   return bytes;
 }
 
-extern "C" int nz_mx4_linear(const void *codes, const void *scales, uint64_t matrices, uint64_t rows,
-                             uint64_t cols, int dtype, const void *x, uint64_t x_stride,
-                             uint64_t n_rows, uint64_t per_input, const void *experts,
-                             const void *bias, void *y, void *workspace, uint64_t workspace_bytes,
-                             void *status, void *stream) {
+extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t rows, uint64_t cols, int dtype,
+                             const void *x, uint64_t x_stride, uint64_t n_rows, uint64_t per_input,
+                             const void *experts, const void *bias, void *y, void *workspace,
+                             uint64_t workspace_bytes, void *status, void *stream) {
   using namespace nz;
   if (!mx_dtype("nz_mx4_linear", dtype) || !mx_shape("nz_mx4_linear", matrices, rows, cols))
     return NZ_E_ARG;
@@ -718,10 +729,10 @@ extern "C" int nz_mx4_linear(const void *codes, const void *scales, uint64_t mat
               (unsigned long long)x_stride);
     return NZ_E_ARG;
   }
-  if (!codes || !scales || !x || !y || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15) ||
+  if (!packed || !x || !y || ((uintptr_t)packed & 15) ||
       ((uintptr_t)x & 1) || ((uintptr_t)y & 1) || ((uintptr_t)bias & 1) || ((uintptr_t)experts & 7) ||
       !workspace || ((uintptr_t)workspace & 255)) {
-    set_error("nz_mx4_linear: null or misaligned pointer (codes and scales 16-byte, experts 8-byte, "
+    set_error("nz_mx4_linear: null or misaligned pointer (stored bytes 16-byte, experts 8-byte, "
               "workspace 256-byte aligned)");
     return NZ_E_ARG;
   }
@@ -736,22 +747,12 @@ extern "C" int nz_mx4_linear(const void *codes, const void *scales, uint64_t mat
               (unsigned long long)workspace_bytes, (unsigned long long)g.bytes);
     return NZ_E_CAPACITY;
   }
-  if (!mx_encode_tiled()) {
-    set_error("nz_mx4_linear: the driver does not provide cuTensorMapEncodeTiled");
-    return NZ_E_CUDA;
-  }
   uint8_t *ws = (uint8_t *)workspace;
-  CUtensorMap w_map, x_map;
-  if (!mx_map(&w_map, codes, matrices * rows, w.code_pitch(), kMxTileRows) ||
-      !mx_map(&x_map, ws + g.x_codes, g.slots * g.tok, w.code_pitch(), g.tok)) {
-    set_error("nz_mx4_linear: cuTensorMapEncodeTiled failed");
-    return NZ_E_CUDA;
-  }
   MxLinearArgs p;
   memset(&p, 0, sizeof(p));
   p.w = w;
-  p.codes = (const uint8_t *)codes;
-  p.scales = (const uint8_t *)scales;
+  p.packed = (const uint8_t *)packed;
+  p.tile_bytes = w.tile_bytes();
   p.x = x;
   p.x_stride = x_stride;
   p.n_rows = (uint32_t)n_rows;
@@ -765,6 +766,8 @@ extern "C" int nz_mx4_linear(const void *codes, const void *scales, uint64_t mat
   p.slots = (uint32_t)g.slots;
   p.row_tiles = g.row_tiles;
   p.steps = g.steps;
+  p.blocks = (uint32_t)w.blocks();
+  p.x_step_bytes = g.x_step_bytes;
   p.split = g.split;
   p.stages = g.stages;
   p.stage_bytes = g.stage_bytes;
@@ -774,9 +777,8 @@ extern "C" int nz_mx4_linear(const void *codes, const void *scales, uint64_t mat
   p.slot_rows = (uint32_t *)(ws + g.slot_rows);
   p.row_of = (uint32_t *)(ws + g.row_of);
   p.place_of = (uint32_t *)(ws + g.place_of);
-  p.x_codes = ws + g.x_codes;
-  p.x_scales = ws + g.x_scales;
+  p.x_packed = ws + g.x_packed;
   p.partial = (float *)(ws + g.partial);
-  return dtype == NZ_DTYPE_BF16 ? mx_launch<__nv_bfloat16>(p, g, w_map, x_map, (cudaStream_t)stream)
-                                : mx_launch<__half>(p, g, w_map, x_map, (cudaStream_t)stream);
+  return dtype == NZ_DTYPE_BF16 ? mx_launch<__nv_bfloat16>(p, g, (cudaStream_t)stream)
+                                : mx_launch<__half>(p, g, (cudaStream_t)stream);
 }

@@ -32,8 +32,7 @@ class _Entry:
     matrices: int             # the stack that is stored: [matrices, rows, cols]
     rows: int
     cols: int
-    codes: torch.Tensor       # uint8
-    scales: torch.Tensor      # uint8
+    packed: torch.Tensor      # uint8: codes and scales in the tensor cores' order
     streams: set = field(default_factory=set)    # streams whose use the allocator knows of
 
     @property
@@ -51,9 +50,8 @@ def _stack(shape: Sequence[int]):
 
 
 @functools.lru_cache(maxsize=512)
-def _sizes(matrices: int, rows: int, cols: int):
-    L = _lib.load()
-    return int(L.nz_mx4_code_bytes(matrices, rows, cols)), int(L.nz_mx4_scale_bytes(matrices, rows, cols))
+def _stored_bytes(matrices: int, rows: int, cols: int) -> int:
+    return int(_lib.load().nz_mx4_bytes(matrices, rows, cols))
 
 
 @functools.lru_cache(maxsize=2048)
@@ -102,12 +100,11 @@ class MX4Backend:
     def _use(self, entry: _Entry) -> int:
         """The current stream of the current device, which must be the entry's; from now on
         the allocator does not hand the entry's memory out while that stream may read it."""
-        device = entry.codes.get_device()
+        device = entry.packed.get_device()
         stream = torch._C._cuda_getCurrentRawStream(device)
         if stream not in entry.streams:
             current = torch.cuda.current_stream(device)
-            entry.codes.record_stream(current)
-            entry.scales.record_stream(current)
+            entry.packed.record_stream(current)
             entry.streams.add(stream)
         return stream
 
@@ -124,16 +121,11 @@ class MX4Backend:
         matrices, rows, cols = _stack(source.shape)
         with torch.cuda.device(device):
             self._status_of(device)
-            code_bytes, scale_bytes = _sizes(matrices, rows, cols)
-            codes = torch.empty(code_bytes, dtype=torch.uint8, device=source.device)
-            # the last row tile's missing rows are never used, but they are part of a checkpoint
-            scales = (torch.zeros if rows % 128 else torch.empty)(
-                scale_bytes, dtype=torch.uint8, device=source.device)
+            packed = torch.empty(_stored_bytes(matrices, rows, cols), dtype=torch.uint8, device=source.device)
             stream = torch._C._cuda_getCurrentRawStream(device)
             _lib.check(self._lib.nz_mx4_quantize(_ptr(source), _DTYPES[tensor.dtype], matrices, rows, cols,
-                                                 _ptr(codes), _ptr(scales), stream))
-        self._cache[name] = _Entry(tensor.shape, tensor.dtype, matrices, rows, cols, codes, scales,
-                                   {stream})
+                                                 _ptr(packed), stream))
+        self._cache[name] = _Entry(tensor.shape, tensor.dtype, matrices, rows, cols, packed, {stream})
 
     def read(self, name: str) -> torch.Tensor:
         """The stored numbers as a flat tensor of the type that was written."""
@@ -142,10 +134,10 @@ class MX4Backend:
 
     def read_shaped(self, name: str, shape) -> torch.Tensor:
         entry = self._get(name)
-        with torch.cuda.device(entry.codes.device):
-            out = torch.empty(entry.numel, dtype=entry.dtype, device=entry.codes.device).view(tuple(shape))
+        with torch.cuda.device(entry.packed.device):
+            out = torch.empty(entry.numel, dtype=entry.dtype, device=entry.packed.device).view(tuple(shape))
             _lib.check(self._lib.nz_mx4_dequantize(
-                _ptr(entry.codes), _ptr(entry.scales), entry.matrices, entry.rows, entry.cols,
+                _ptr(entry.packed), entry.matrices, entry.rows, entry.cols,
                 _DTYPES[entry.dtype], _ptr(out), self._use(entry)))
         return out
 
@@ -161,7 +153,7 @@ class MX4Backend:
             raise ValueError(f"row length {row_len} does not divide the {entry.numel} stored elements")
         if rows.is_floating_point() or rows.is_complex() or rows.dtype == torch.bool:
             raise TypeError(f"row numbers must be integers, got {rows.dtype}")
-        device = entry.codes.device
+        device = entry.packed.device
         rows = rows.reshape(-1).to(device=device, dtype=torch.int64).contiguous()
         if row_len != entry.cols:
             # rows of several dimensions: each is a run of the table's own rows
@@ -172,7 +164,7 @@ class MX4Backend:
         with torch.cuda.device(device):
             out = torch.empty(rows.numel(), entry.cols, dtype=entry.dtype, device=device)
             _lib.check(self._lib.nz_mx4_gather_rows(
-                _ptr(entry.codes), _ptr(entry.scales), entry.matrices, entry.rows, entry.cols,
+                _ptr(entry.packed), entry.matrices, entry.rows, entry.cols,
                 _DTYPES[entry.dtype], _ptr(rows), rows.numel(), _ptr(out),
                 _ptr(self._status_of(device.index)), self._use(entry)))
         return out.view(-1, row_len)
@@ -180,7 +172,7 @@ class MX4Backend:
     def size(self, name: str) -> int:
         """Stored bytes, 0 for an unknown name."""
         entry = self._cache.get(name)
-        return 0 if entry is None else entry.codes.numel() + entry.scales.numel()
+        return 0 if entry is None else entry.packed.numel()
 
     def linear(self, name: str, input: torch.Tensor, shape: Sequence[int],
                bias: Optional[torch.Tensor]) -> torch.Tensor:
@@ -213,8 +205,8 @@ class MX4Backend:
                              f"got a tensor of shape {tuple(entry.shape)}")
         if experts.is_floating_point() or experts.is_complex() or experts.dtype == torch.bool:
             raise TypeError(f"expert numbers must be integers, got {experts.dtype}")
-        if experts.device != entry.codes.device:
-            raise ValueError(f"expert numbers are on {experts.device}, the weights on {entry.codes.device}")
+        if experts.device != entry.packed.device:
+            raise ValueError(f"expert numbers are on {experts.device}, the weights on {entry.packed.device}")
         lead, per_input = input.shape[:-1], 1
         if lead != experts.shape:
             if experts.dim() == 0 or lead != experts.shape[:-1]:
@@ -235,8 +227,8 @@ class MX4Backend:
         if input.dim() < 1 or input.shape[-1] != entry.cols or entry.cols == 0:
             raise ValueError(f"inputs of shape {tuple(input.shape)} do not fit weights of shape "
                              f"{tuple(entry.shape)}")
-        if input.device != entry.codes.device:
-            raise ValueError(f"inputs are on {input.device}, the weights on {entry.codes.device}")
+        if input.device != entry.packed.device:
+            raise ValueError(f"inputs are on {input.device}, the weights on {entry.packed.device}")
         if bias is not None and (bias.dtype != input.dtype or bias.device != input.device
                                  or bias.numel() != entry.matrices * entry.rows):
             raise ValueError(f"bias must be {entry.matrices * entry.rows} numbers of type "
@@ -263,7 +255,7 @@ class MX4Backend:
         workspace = torch.empty(_workspace_bytes(device, entry.matrices, entry.rows, entry.cols, n_rows),
                                 dtype=torch.uint8, device=x.device)
         rc = self._lib.nz_mx4_linear(
-            _ptr(entry.codes), _ptr(entry.scales), entry.matrices, entry.rows, entry.cols,
+            _ptr(entry.packed), entry.matrices, entry.rows, entry.cols,
             _DTYPES[x.dtype], _ptr(x), x.stride(0), n_rows, per_input, _ptr(ids), _ptr(bias), _ptr(y),
             _ptr(workspace), workspace.numel(), _ptr(self._status_of(device)), self._use(entry))
         if rc:
@@ -277,7 +269,7 @@ class MX4Backend:
         """The stored form of one tensor as CPU tensors plus what is needed to read it."""
         e = self._cache[name]
         return {"format": "MXFP4", "dtype": _NAMES[e.dtype], "stack": (e.matrices, e.rows, e.cols),
-                "codes": e.codes.cpu(), "scales": e.scales.cpu()}
+                "packed": e.packed.cpu()}
 
     def import_entry(self, name: str, blob: dict) -> None:
         """Inverse of `export_entry`: the stored bytes go straight to the GPU."""
@@ -288,13 +280,12 @@ class MX4Backend:
         dtype = {v: k for k, v in _NAMES.items()}.get(blob["dtype"])
         if dtype is None or tuple(blob["stack"]) != stack:
             raise ValueError("checkpoint entry: type or shape does not fit the stored bytes")
-        if (blob["codes"].numel(), blob["scales"].numel()) != _sizes(*stack):
-            raise ValueError("checkpoint entry: codes or scales have the wrong length")
-        codes = blob["codes"].to(device="cuda", dtype=torch.uint8).contiguous()
-        scales = blob["scales"].to(device="cuda", dtype=torch.uint8).contiguous()
-        device = codes.get_device()
+        if blob["packed"].numel() != _stored_bytes(*stack):
+            raise ValueError("checkpoint entry: the stored bytes have the wrong length")
+        packed = blob["packed"].to(device="cuda", dtype=torch.uint8).contiguous()
+        device = packed.get_device()
         self._status_of(device)
-        self._cache[name] = _Entry(shape, dtype, *stack, codes, scales,
+        self._cache[name] = _Entry(shape, dtype, *stack, packed,
                                    {torch._C._cuda_getCurrentRawStream(device)})
 
     # -- extras -----------------------------------------------------------

@@ -14,8 +14,7 @@ def manager_with(shape, name="w"):
     stack = _stack(shape)
     L = _lib.load()
     m._be._cache[name] = _Entry(torch.Size(shape), torch.bfloat16, *stack,
-                                torch.zeros(int(L.nz_mx4_code_bytes(*stack)), dtype=torch.uint8),
-                                torch.zeros(int(L.nz_mx4_scale_bytes(*stack)), dtype=torch.uint8))
+                                torch.zeros(int(L.nz_mx4_bytes(*stack)), dtype=torch.uint8))
     m.meta_dict[name] = torch.Size(shape)
     return m
 
@@ -25,21 +24,20 @@ def test_names():
     assert "MX4Manager" in neuzip.__all__ and neuzip.nn.Experts
 
 
-@pytest.mark.parametrize("shape,stack,codes,scales", [
-    ((4096, 4096), (1, 4096, 4096), 4096 * 2048, 4096 * 128),
-    ((1, 1), (1, 1, 1), 16, 1024),
-    ((129, 257), (1, 129, 257), 129 * 144, 2 * 2 * 1024),
-    ((3, 5, 33), (3, 5, 33), 15 * 32, 3 * 1024),
-    ((2, 3, 4, 64), (1, 24, 64), 24 * 32, 1024),
-    ((), (1, 1, 1), 16, 1024),
-    ((0, 64), (1, 0, 64), 0, 0),
-    ((7,), (1, 1, 7), 16, 1024),
+@pytest.mark.parametrize("shape,stack,tiles,blocks,steps", [
+    ((4096, 4096), (1, 4096, 4096), 32, 128, 16),
+    ((1, 1), (1, 1, 1), 1, 1, 1),
+    ((129, 257), (1, 129, 257), 2, 9, 2),
+    ((3, 5, 33), (3, 5, 33), 3, 2, 1),
+    ((2, 3, 4, 64), (1, 24, 64), 1, 2, 1),
+    ((), (1, 1, 1), 1, 1, 1),
+    ((0, 64), (1, 0, 64), 0, 2, 1),
+    ((7,), (1, 1, 7), 1, 1, 1),
 ])
-def test_sizes(shape, stack, codes, scales):
-    L = _lib.load()
+def test_sizes(shape, stack, tiles, blocks, steps):
+    # a tile of 128 rows: 16 bytes a row and block, a kilobyte of scales for every 256 columns
     assert _stack(shape) == stack
-    assert L.nz_mx4_code_bytes(*stack) == codes
-    assert L.nz_mx4_scale_bytes(*stack) == scales
+    assert _lib.load().nz_mx4_bytes(*stack) == tiles * (blocks * 2048 + steps * 1024)
 
 
 def test_reference_rounds_to_the_nearest_code():
@@ -140,31 +138,31 @@ def test_experts_refuses():
 def test_import_refuses_what_does_not_fit():
     m = neuzip.MX4Manager()
     blob = {"format": "MXFP4", "dtype": "bfloat16", "shape": (4, 64), "stack": (1, 4, 64),
-            "codes": torch.zeros(128, dtype=torch.uint8), "scales": torch.zeros(1024, dtype=torch.uint8)}
+            "packed": torch.zeros(2 * 2048 + 1024, dtype=torch.uint8)}
     for change in ({"format": "NZR1"}, {"dtype": "float32"}, {"shape": (4, 65)},
-                   {"codes": torch.zeros(127, dtype=torch.uint8)},
-                   {"scales": torch.zeros(512, dtype=torch.uint8)}):
+                   {"packed": torch.zeros(5119, dtype=torch.uint8)}):
         with pytest.raises(ValueError):
             m.import_entry({**blob, **change}, "w")
 
 
 def test_library_refuses_bad_arguments():
     L = _lib.load()
-    assert L.nz_mx4_quantize(0, 2, 1, 1, 1, 0, 0, 0) == _lib.NZ_E_ARG
-    assert L.nz_mx4_quantize(0, 0, 1, 1, 1, 0, 0, 0) == _lib.NZ_E_ARG
-    assert L.nz_mx4_quantize(0, 0, 1, 1 << 31, 1, 0, 0, 0) == _lib.NZ_E_ARG
-    assert L.nz_mx4_dequantize(0, 0, 1, 1, 1, 7, 0, 0) == _lib.NZ_E_ARG
-    assert L.nz_mx4_dequantize(16, 16, 1, 1, 1, 0, 0, 0) == _lib.NZ_E_ARG
-    assert L.nz_mx4_gather_rows(16, 16, 1, 1, 1, 0, 0, 1, 16, 0, 0) == _lib.NZ_E_ARG
-    # product: codes, scales, matrices, rows, cols, dtype, x, stride, n_rows, per_input, experts, bias,
+    assert L.nz_mx4_quantize(0, 2, 1, 1, 1, 0, 0) == _lib.NZ_E_ARG
+    assert L.nz_mx4_quantize(0, 0, 1, 1, 1, 0, 0) == _lib.NZ_E_ARG
+    assert L.nz_mx4_quantize(0, 0, 1, 1 << 31, 1, 0, 0) == _lib.NZ_E_ARG
+    assert L.nz_mx4_quantize(16, 0, 1, 1, 1, 8, 0) == _lib.NZ_E_ARG
+    assert L.nz_mx4_dequantize(0, 1, 1, 1, 7, 0, 0) == _lib.NZ_E_ARG
+    assert L.nz_mx4_dequantize(16, 1, 1, 1, 0, 0, 0) == _lib.NZ_E_ARG
+    assert L.nz_mx4_gather_rows(16, 1, 1, 1, 0, 0, 1, 16, 0, 0) == _lib.NZ_E_ARG
+    # product: stored bytes, matrices, rows, cols, dtype, x, stride, n_rows, per_input, experts, bias,
     # y, workspace, bytes, status, stream
-    good = [16, 16, 1, 8, 64, 0, 16, 64, 4, 1, 0, 0, 16, 256, 1 << 30, 16, 0]
-    for at, value in ((0, 0), (0, 8), (1, 0), (3, 1 << 31), (5, 3), (6, 0), (6, 1), (7, 63), (9, 0),
-                      (9, 3), (2, 2), (12, 0), (13, 0), (13, 16), (8, 1 << 31), (11, 1), (10, 4)):
+    good = [16, 1, 8, 64, 0, 16, 64, 4, 1, 0, 0, 16, 256, 1 << 30, 16, 0]
+    for at, value in ((0, 0), (0, 8), (2, 1 << 31), (4, 3), (5, 0), (5, 1), (6, 63), (8, 0), (8, 3), (1, 2),
+                      (11, 0), (12, 0), (12, 16), (7, 1 << 31), (10, 1), (9, 4)):
         bad = list(good)
         bad[at] = value
         assert L.nz_mx4_linear(*bad) == _lib.NZ_E_ARG, (at, value)
     bad = list(good)
-    bad[14] = 0
+    bad[13] = 0
     assert L.nz_mx4_linear(*bad) == _lib.NZ_E_CAPACITY
-    assert L.nz_mx4_linear(*([0] * 3 + [8, 64, 0] + [0] * 11)) == _lib.NZ_OK      # no rows: nothing to do
+    assert L.nz_mx4_linear(*([0, 0, 8, 64] + [0] * 12)) == _lib.NZ_OK      # no rows: nothing to do
