@@ -40,6 +40,34 @@ mx4_quantize_kernel(const T *__restrict__ in, MxShape s, uint8_t *__restrict__ p
   }
 }
 
+// Where the codes and the scale of a block of a row lie.
+struct MxPlace {
+  const uint8_t *codes, *scale;
+};
+__device__ __forceinline__ MxPlace mx_place(const uint8_t *packed, const MxShape &s, uint64_t row, uint32_t block) {
+  const uint64_t matrix = s.matrices == 1 ? 0 : row / s.rows;
+  const uint32_t r = (uint32_t)(row - matrix * s.rows), blocks = (uint32_t)s.blocks(), first = block & ~7u;
+  const uint8_t *step = packed + (matrix * s.row_tiles() + r / kMxTileRows) * s.tile_bytes() +
+                        (uint64_t)(block >> 3) * kMxStepBytes;
+  const uint32_t held = blocks - first < 8 ? blocks - first : 8;
+  return {step + (block - first) * kMxBlockBytes + (r % kMxTileRows) * 16,
+          step + held * kMxBlockBytes + mx_scale_offset(r % kMxTileRows, block & 7u, 1)};
+}
+// The row of the stack that is row `to` of the output; false (and a status bit) where the list names
+// none.
+__device__ __forceinline__ bool mx_listed(const int64_t *list, const MxShape &s, uint64_t to, uint64_t &row,
+                                          uint32_t *status) {
+  row = to;
+  if (!list) return true;
+  const int64_t want = __ldg(list + to);
+  if (want >= 0 && (uint64_t)want < s.matrices * s.rows) {
+    row = (uint64_t)want;
+    return true;
+  }
+  if (status) atomicOr(status, NZ_STATUS_BAD_INDEX);
+  return false;
+}
+
 // The way back, the same items.  With a list, output row i is row list[i] of the stack (zeros and a
 // status bit where there is no such row).
 template <typename T, int WIDE>
@@ -49,30 +77,18 @@ mx4_dequantize_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
   const uint32_t blocks = (uint32_t)s.blocks(), quads = (blocks + 3) / 4;
-  const uint64_t tile_bytes = s.tile_bytes(), total = (out_rows + 7) / 8 * quads;
+  const uint64_t total = (out_rows + 7) / 8 * quads;
   for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
     const uint64_t group = w / quads, to = group * 8 + (lane & 7u);
     const uint32_t block = (uint32_t)(w - group * quads) * 4 + (lane >> 3);
     if (block >= blocks || to >= out_rows) continue;
-    uint64_t row = to;
-    bool there = true;
-    if (list) {
-      const int64_t want = list[to];
-      there = want >= 0 && (uint64_t)want < s.matrices * s.rows;
-      row = there ? (uint64_t)want : 0;
-      if (!there && block == 0 && status) atomicOr(status, NZ_STATUS_BAD_INDEX);
-    }
+    uint64_t row;
     uint4 code = make_uint4(0, 0, 0, 0);
     uint32_t byte = 0;
-    if (there) {
-      const uint64_t matrix = s.matrices == 1 ? 0 : row / s.rows;
-      const uint32_t r = (uint32_t)(row - matrix * s.rows), first = block & ~7u;
-      const uint8_t *step = packed + (matrix * s.row_tiles() + r / kMxTileRows) * tile_bytes +
-                            (uint64_t)(block >> 3) * kMxStepBytes;
-      const uint32_t held = blocks - first < 8 ? blocks - first : 8;
-      code = __ldg(reinterpret_cast<const uint4 *>(step + (block - first) * kMxBlockBytes +
-                                                   (r % kMxTileRows) * 16));
-      byte = __ldg(step + held * kMxBlockBytes + mx_scale_offset(r % kMxTileRows, block & 7u, 1));
+    if (mx_listed(list, s, to, row, status)) {
+      const MxPlace at = mx_place(packed, s, row, block);
+      code = __ldg(reinterpret_cast<const uint4 *>(at.codes));
+      byte = __ldg(at.scale);
     }
     const float scale = mx_scale(byte);
     const uint32_t c[4] = {code.x, code.y, code.z, code.w};
@@ -93,18 +109,47 @@ mx4_dequantize_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64
                        "r"(v[8 * h]), "r"(v[8 * h + 1]), "r"(v[8 * h + 2]), "r"(v[8 * h + 3]),
                        "r"(v[8 * h + 4]), "r"(v[8 * h + 5]), "r"(v[8 * h + 6]), "r"(v[8 * h + 7])
                        : "memory");
-    } else if (WIDE == 1) {
+    } else {
 #pragma unroll
       for (int h = 0; h < 4; ++h)
         if (left > 8 * h)
           *reinterpret_cast<uint4 *>(dst + 8 * h) = make_uint4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-    } else {
+    }
+  }
+}
+
+// The same where rows of the output are not aligned: a warp takes a row of up to eight blocks and
+// a lane one element of each, so that every store is 64 bytes in a piece (a block per thread, two
+// bytes at a time: 75 instead of 8 us for 1001 x 4099).
+template <typename T>
+__global__ void __launch_bounds__(kMxThreads)
+mx4_dequantize_odd_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64_t *__restrict__ list,
+                          uint64_t out_rows, T *__restrict__ out, uint32_t *status) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
+  const uint32_t blocks = (uint32_t)s.blocks(), steps = (uint32_t)s.steps();
+  const uint64_t total = out_rows * steps;
+  for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
+    const uint64_t to = w / steps;
+    const uint32_t first = (uint32_t)(w - to * steps) * 8;
+    uint64_t row;
+    const bool there = mx_listed(list, s, to, row, status);
+    uint32_t code[8], byte[8];
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < left) {
-          const uint16_t bits = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
-          memcpy(dst + i, &bits, 2);
-        }
+    for (uint32_t b = 0; b < 8; ++b) {
+      code[b] = byte[b] = 0;
+      if (there && first + b < blocks) {
+        const MxPlace at = mx_place(packed, s, row, first + b);
+        code[b] = __ldg(at.codes + (lane >> 1));
+        byte[b] = __ldg(at.scale);
+      }
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < 8; ++b) {
+      const uint64_t col = (uint64_t)(first + b) * kMxBlock + lane;
+      if (col >= s.cols) break;
+      const float2 f = mx_decode2(code[b]);
+      out[to * s.cols + col] = from_float<T>(((lane & 1u) ? f.y : f.x) * mx_scale(byte[b]));
     }
   }
 }
@@ -171,10 +216,10 @@ template <typename T>
 static int dequantize(const void *packed, const nz::MxShape &s, const void *list, uint64_t out_rows,
                       void *out, void *status, cudaStream_t st) {
   using namespace nz;
-  const uint64_t warps = (out_rows + 7) / 8 * ((s.blocks() + 3) / 4);
   const int wide = mx_wide(out, s.cols);
+  const uint64_t warps = wide ? (out_rows + 7) / 8 * ((s.blocks() + 3) / 4) : out_rows * s.steps();
   auto kern = wide == 2 ? mx4_dequantize_kernel<T, 2> : wide == 1 ? mx4_dequantize_kernel<T, 1>
-                                                                  : mx4_dequantize_kernel<T, 0>;
+                                                                  : mx4_dequantize_odd_kernel<T>;
   kern<<<mx_grid(warps), kMxThreads, 0, st>>>((const uint8_t *)packed, s, (const int64_t *)list, out_rows,
                                               (T *)out, (uint32_t *)status);
   NZ_LAUNCH_CHECK("mx4_dequantize_kernel");

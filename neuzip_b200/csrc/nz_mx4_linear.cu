@@ -46,6 +46,7 @@ struct MxLinearArgs {
   uint32_t x_step_bytes;      // a step of a slot: codes, scales
   uint32_t split;             // 1: the steps of a tile may be shared between CTAs
   uint32_t stages, stage_bytes;
+  uint32_t wide_y;            // 1: rows of y are whole 16-byte pieces
   // workspace
   uint32_t *n_slots;          // stack: slots that there are
   uint32_t *counters;         // split: arrivals at every tile
@@ -326,8 +327,9 @@ struct MxItems {
 constexpr uint32_t kMxBarFull = 0, kMxBarEmpty = 8 * kMxMaxStages, kMxBarAccFull = 16 * kMxMaxStages,
                    kMxBarAccEmpty = kMxBarAccFull + 16, kMxBarDrain = kMxBarAccEmpty + 16,
                    kMxTmemSlot = kMxBarDrain + 8,
-                   kMxAbortSlot = kMxTmemSlot + 4, kMxLastSlot = kMxAbortSlot + 4, kMxMiscBytes = 256;
-static_assert(kMxLastSlot + 4 <= kMxMiscBytes, "barriers");
+                   kMxAbortSlot = kMxTmemSlot + 4, kMxLastSlot = kMxAbortSlot + 4, kMxTurn = 256,
+                   kMxMiscBytes = kMxTurn + 4 * 1024;      // 16 rows x 32 features of y for each storing warp
+static_assert(kMxLastSlot + 4 <= kMxTurn, "barriers");
 
 template <typename T>
 __global__ void __launch_bounds__(kMxLinThreads, 1)
@@ -476,6 +478,7 @@ mx4_product_kernel(const MxLinearArgs p) {
   } else {
     // ---------------------------------------------------------------- results
     const uint32_t sub = warp & 3u;                   // tensor-memory lanes 32 sub .. + 31
+    T *turn = reinterpret_cast<T *>(misc + kMxTurn) + sub * 512;
     uint32_t item = 0;
     MxItem it;
     while (items.next(it)) {
@@ -483,7 +486,31 @@ mx4_product_kernel(const MxLinearArgs p) {
       const uint32_t feature = it.row_tile * kMxTileRows + 32 * sub + lane;
       const bool real = feature < p.w.rows;
       const float bias = p.bias && real ? to_float<T>(((const T *)p.bias)[it.expert * p.w.rows + feature]) : 0.f;
-      T *y = (T *)p.y + feature;
+      // 16 rows of y of this warp's 32 features, from a value for every row in each lane
+      T *y = (T *)p.y + it.row_tile * kMxTileRows + 32 * sub;
+      auto store16 = [&](const float (&f)[16], uint32_t row_here, uint32_t count) {
+        if (p.wide_y) {
+          // turned in shared memory: four lanes take a row's 64 bytes
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) turn[i * 32 + lane] = from_float<T>(f[i] + bias);
+          __syncwarp();
+          const bool in = it.row_tile * kMxTileRows + 32 * sub + 8 * (lane & 3u) < p.w.rows;
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t i = 8 * h + (lane >> 2);
+            const uint64_t r = __shfl_sync(0xFFFFFFFFu, row_here, i);
+            const uint4 piece = *reinterpret_cast<const uint4 *>(turn + i * 32 + 8 * (lane & 3u));
+            if (i < count && in) *reinterpret_cast<uint4 *>(y + r * p.w.rows + 8 * (lane & 3u)) = piece;
+          }
+          __syncwarp();
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) {
+            const uint64_t r = __shfl_sync(0xFFFFFFFFu, row_here, i);
+            if (i < count && real) y[r * p.w.rows + lane] = from_float<T>(f[i] + bias);
+          }
+        }
+      };
       // lane i of 16 knows the row of y of column c0 + i; fetched 16 columns ahead
       auto row_at = [&](uint32_t c) -> uint32_t {
         if (!p.experts) return place0 + c + (lane & 15u);
@@ -511,15 +538,15 @@ mx4_product_kernel(const MxLinearArgs p) {
           __syncwarp();
           if (lane == 0) mx_mbar_arrive(misc_a + kMxBarAccEmpty + 8 * acc);
         }
+        if (!whole) {
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-          if (c0 + i >= rows) break;
-          if (!whole) {
-            piece[(uint64_t)(c0 + i) * kMxTileRows] = __uint_as_float(v[i]);
-          } else {
-            const uint64_t r = __shfl_sync(0xFFFFFFFFu, row_here, i);
-            if (real) y[r * p.w.rows] = from_float<T>(__uint_as_float(v[i]) + bias);
-          }
+          for (uint32_t i = 0; i < 16; ++i)
+            if (c0 + i < rows) piece[(uint64_t)(c0 + i) * kMxTileRows] = __uint_as_float(v[i]);
+        } else {
+          float f[16];
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+          store16(f, row_here, rows - c0);
         }
       }
       if (!whole) {
@@ -534,29 +561,23 @@ mx4_product_kernel(const MxLinearArgs p) {
         mx_store_barrier();
         if (*last_flag) {
           const float *from = p.partial + (uint64_t)it.tile * items.pieces * p.tok * kMxTileRows + 32 * sub + lane;
-          constexpr uint32_t kCols = 8, kPieces = 4;      // loads in flight
-          for (uint32_t c0 = 0; c0 < rows; c0 += kCols) {
-            float sum[kCols] = {};
-            const uint32_t row_here = row_at(c0 & ~15u);
-            for (uint32_t q0 = 0; q0 < items.pieces; q0 += kPieces) {
-              float add[kPieces][kCols];
+          for (uint32_t c0 = 0; c0 < rows; c0 += 16) {
+            float sum[16] = {};
+            const uint32_t row_here = row_at(c0);
+            for (uint32_t q0 = 0; q0 < items.pieces; q0 += 4) {
+              float add[4][16];                       // loads in flight
 #pragma unroll
-              for (uint32_t q = 0; q < kPieces; ++q)
+              for (uint32_t q = 0; q < 4; ++q)
 #pragma unroll
-                for (uint32_t i = 0; i < kCols; ++i)
+                for (uint32_t i = 0; i < 16; ++i)
                   add[q][i] = q0 + q < items.pieces && c0 + i < rows
                                   ? __ldcg(from + ((uint64_t)(q0 + q) * p.tok + c0 + i) * kMxTileRows) : 0.f;
 #pragma unroll
-              for (uint32_t q = 0; q < kPieces; ++q)
+              for (uint32_t q = 0; q < 4; ++q)
 #pragma unroll
-                for (uint32_t i = 0; i < kCols; ++i) sum[i] += add[q][i];
+                for (uint32_t i = 0; i < 16; ++i) sum[i] += add[q][i];
             }
-#pragma unroll
-            for (uint32_t i = 0; i < kCols; ++i) {
-              if (c0 + i >= rows) break;
-              const uint64_t r = __shfl_sync(0xFFFFFFFFu, row_here, (c0 & 15u) + i);
-              if (real) y[r * p.w.rows] = from_float<T>(sum[i] + bias);
-            }
+            store16(sum, row_here, rows - c0);
           }
         }
       }
@@ -771,6 +792,7 @@ extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t row
   p.split = g.split;
   p.stages = g.stages;
   p.stage_bytes = g.stage_bytes;
+  p.wide_y = rows % 8 == 0 && ((uintptr_t)y & 15) == 0;
   p.n_slots = (uint32_t *)ws;
   p.counters = (uint32_t *)(ws + g.counters);
   p.slot_expert = (uint32_t *)(ws + g.slot_expert);
