@@ -123,7 +123,7 @@ SIGNATURES["nz_mx4_bytes"] = (_u64, [_u64, _u64, _u64])
 SIGNATURES["nz_mx4_quantize"] = (_int, [_vp, _int, _u64, _u64, _u64, _vp, _vp])
 SIGNATURES["nz_mx4_dequantize"] = (_int, [_vp, _u64, _u64, _u64, _int, _vp, _vp])
 SIGNATURES["nz_mx4_gather_rows"] = (_int, [_vp, _u64, _u64, _u64, _int, _vp, _u64, _vp, _vp, _vp])
-SIGNATURES["nz_mx4_linear_workspace_bytes"] = (_u64, [_u64, _u64, _u64, _u64])
+SIGNATURES["nz_mx4_linear_workspace_bytes"] = (_u64, [_u64, _u64, _u64, _u64, _int])
 SIGNATURES["nz_mx4_linear"] = (
     _int, [_vp, _u64, _u64, _u64, _int, _vp, _u64, _u64, _u64, _vp, _vp, _vp, _vp, _u64, _vp, _vp])
 

@@ -174,11 +174,6 @@ static unsigned mx_grid(uint64_t warps) {
   const uint64_t most = (uint64_t)sm_count() * 8;            // 2048 threads an SM
   return (unsigned)(blocks < most ? blocks : most);
 }
-// How wide the rows of a contiguous tensor can be read or written.
-static int mx_wide(const void *p, uint64_t cols) {
-  return cols % 16 == 0 && ((uintptr_t)p & 31) == 0 ? 2 : cols % 8 == 0 && ((uintptr_t)p & 15) == 0 ? 1 : 0;
-}
-
 }  // namespace nz
 
 extern "C" uint64_t nz_mx4_bytes(uint64_t matrices, uint64_t rows, uint64_t cols) {
@@ -189,7 +184,7 @@ template <typename T>
 static int quantize(const void *in, const nz::MxShape &s, void *packed, cudaStream_t st) {
   using namespace nz;
   const uint64_t warps = s.matrices * s.row_tiles() * (kMxTileRows / 8) * 2 * s.steps();
-  const int wide = mx_wide(in, s.cols);
+  const int wide = mx_wide_rows(in, s.cols, s.cols);
   auto kern = wide == 2 ? mx4_quantize_kernel<T, 2> : wide == 1 ? mx4_quantize_kernel<T, 1>
                                                                 : mx4_quantize_kernel<T, 0>;
   kern<<<mx_grid(warps), kMxThreads, 0, st>>>((const T *)in, s, (uint8_t *)packed);
@@ -216,7 +211,7 @@ template <typename T>
 static int dequantize(const void *packed, const nz::MxShape &s, const void *list, uint64_t out_rows,
                       void *out, void *status, cudaStream_t st) {
   using namespace nz;
-  const int wide = mx_wide(out, s.cols);
+  const int wide = mx_wide_rows(out, s.cols, s.cols);
   const uint64_t warps = wide ? (out_rows + 7) / 8 * ((s.blocks() + 3) / 4) : out_rows * s.steps();
   auto kern = wide == 2 ? mx4_dequantize_kernel<T, 2> : wide == 1 ? mx4_dequantize_kernel<T, 1>
                                                                   : mx4_dequantize_odd_kernel<T>;

@@ -97,6 +97,17 @@ __device__ __forceinline__ float2 mx_decode2(uint32_t byte) {
 bool mx_shape(const char *who, uint64_t matrices, uint64_t rows, uint64_t cols);
 bool mx_dtype(const char *who, int dtype);
 
+// How wide rows of 16-bit elements can be read (see mx_load_block).
+inline int mx_wide_rows(const void *p, uint64_t stride, uint64_t cols) {
+  const uint64_t apart = (uint64_t)(uintptr_t)p | stride * 2 | cols * 2;
+  return apart % 32 == 0 ? 2 : apart % 16 == 0 ? 1 : 0;
+}
+
+// The product for few rows (nz_mx4_few.cu): whether it takes a call, and the call.
+bool mx_few_rows(const MxShape &w, uint64_t n_rows, bool grouped);
+int mx_few(const MxShape &w, int dtype, const void *packed, const void *x, uint64_t x_stride, uint64_t n_rows,
+           uint64_t per_input, const void *experts, const void *bias, void *y, void *status, cudaStream_t st);
+
 // Offset of the scale of row r (in a tile of up to 128 * chunks rows), block b of the step.
 __host__ __device__ __forceinline__ uint32_t mx_scale_offset(uint32_t r, uint32_t b, uint32_t chunks) {
   return ((b >> 2) * chunks + (r >> 7)) * kMxChunk + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (b & 3u);

@@ -687,13 +687,13 @@ template <typename T>
 static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
   static bool product_done[kMaxDeviceOrdinals] = {}, route_done[kMaxDeviceOrdinals] = {};
   NZ_CUDA_TRY(mx_opt_in(mx4_product_kernel<T>, (int)kMaxDynamicSmem, product_done));
-  const uintptr_t apart = (uintptr_t)p.x | (uintptr_t)(p.x_stride * 2) | (uintptr_t)(p.w.cols * 2);
+  const int wide = mx_wide_rows(p.x, p.x_stride, p.w.cols);
   const uint64_t warps = (uint64_t)((p.n_rows / p.per_input + 7) / 8) * 2 * p.steps, blocks = (warps + 7) / 8;
   const unsigned most = (unsigned)sm_count() * 8;
   const unsigned grid = blocks < most ? (unsigned)blocks : most;
-  auto rows_kernel = apart % 32 == 0   ? mx4_quantize_rows_kernel<T, 2>
-                     : apart % 16 == 0 ? mx4_quantize_rows_kernel<T, 1>
-                                       : mx4_quantize_rows_kernel<T, 0>;
+  auto rows_kernel = wide == 2   ? mx4_quantize_rows_kernel<T, 2>
+                     : wide == 1 ? mx4_quantize_rows_kernel<T, 1>
+                                 : mx4_quantize_rows_kernel<T, 0>;
   if (p.experts) {
     NZ_CUDA_TRY(mx_opt_in(mx4_route_kernel, (int)(kMxMaxExperts * 8), route_done));
     mx4_route_kernel<<<1, kMxRouteThreads, p.w.matrices * 8, st>>>(p);
@@ -711,15 +711,14 @@ static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
 }  // namespace nz
 
 extern "C" uint64_t nz_mx4_linear_workspace_bytes(uint64_t matrices, uint64_t rows, uint64_t cols,
-                                                  uint64_t n_rows) {
+                                                  uint64_t n_rows, int grouped) {
   using namespace nz;
-  if (matrices == 0 || rows == 0 || cols == 0 || n_rows == 0) return 256;
-  MxPlan one, many;
   const MxShape w{matrices, rows, cols};
-  uint64_t bytes = 256;
-  if (matrices == 1 && mx_plan(w, n_rows, false, one)) bytes = one.bytes;
-  if (mx_plan(w, n_rows, true, many) && many.bytes > bytes) bytes = many.bytes;
-  return bytes;
+  MxPlan g;
+  if (matrices == 0 || rows == 0 || cols == 0 || n_rows == 0 || mx_few_rows(w, n_rows, grouped != 0) ||
+      !mx_plan(w, n_rows, grouped != 0, g))
+    return 0;
+  return g.bytes;
 }
 
 extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t rows, uint64_t cols, int dtype,
@@ -752,18 +751,21 @@ extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t row
   }
   if (!packed || !x || !y || ((uintptr_t)packed & 15) ||
       ((uintptr_t)x & 1) || ((uintptr_t)y & 1) || ((uintptr_t)bias & 1) || ((uintptr_t)experts & 7) ||
-      !workspace || ((uintptr_t)workspace & 255)) {
+      ((uintptr_t)workspace & 255)) {
     set_error("nz_mx4_linear: null or misaligned pointer (stored bytes 16-byte, experts 8-byte, "
               "workspace 256-byte aligned)");
     return NZ_E_ARG;
   }
   const MxShape w{matrices, rows, cols};
+  if (mx_few_rows(w, n_rows, experts != nullptr))
+    return mx_few(w, dtype, packed, x, x_stride, n_rows, per_input, experts, bias, y, status,
+                  (cudaStream_t)stream);
   MxPlan g;
   if (!mx_plan(w, n_rows, experts != nullptr, g)) {
     set_error("nz_mx4_linear: the product of %llu rows is too large for one call", (unsigned long long)n_rows);
     return NZ_E_ARG;
   }
-  if (workspace_bytes < g.bytes) {
+  if (!workspace || workspace_bytes < g.bytes) {
     set_error("nz_mx4_linear: workspace of %llu bytes is smaller than the %llu required",
               (unsigned long long)workspace_bytes, (unsigned long long)g.bytes);
     return NZ_E_CAPACITY;

@@ -55,8 +55,8 @@ def _stored_bytes(matrices: int, rows: int, cols: int) -> int:
 
 
 @functools.lru_cache(maxsize=2048)
-def _workspace_bytes(device: int, matrices: int, rows: int, cols: int, n_rows: int) -> int:
-    return int(_lib.load().nz_mx4_linear_workspace_bytes(matrices, rows, cols, n_rows))
+def _workspace_bytes(device: int, matrices: int, rows: int, cols: int, n_rows: int, grouped: bool) -> int:
+    return int(_lib.load().nz_mx4_linear_workspace_bytes(matrices, rows, cols, n_rows, grouped))
 
 
 class MX4Backend:
@@ -184,7 +184,7 @@ class MX4Backend:
             raise ValueError(f"linear needs a matrix, got a tensor of shape {tuple(shape)}")
         x = self._checked_input(entry, input, bias)
         n_rows = x.shape[0]
-        y = torch.empty(input.shape[:-1] + (entry.rows,), dtype=input.dtype, device=input.device)
+        y = input.new_empty((*input.shape[:-1], entry.rows))
         self._launch(entry, x, n_rows, 1, None, bias, y)
         return y
 
@@ -214,8 +214,8 @@ class MX4Backend:
                                  f"{tuple(experts.shape)}")
             per_input = int(experts.shape[-1])
         x = self._checked_input(entry, input, bias)
-        ids = experts.to(torch.int64).contiguous()
-        y = torch.empty(experts.shape + (entry.rows,), dtype=input.dtype, device=input.device)
+        ids = (experts if experts.dtype == torch.int64 else experts.long()).contiguous()
+        y = input.new_empty((*experts.shape, entry.rows))
         self._launch(entry, x, ids.numel(), per_input, ids, bias, y)
         return y
 
@@ -251,13 +251,13 @@ class MX4Backend:
                 return self._launch(entry, x, n_rows, per_input, ids, bias, y)
         if bias is not None:
             bias = bias.contiguous()
+        need = _workspace_bytes(device, entry.matrices, entry.rows, entry.cols, n_rows, ids is not None)
         # from the allocator on every call: calls on other streams and captured graphs have their own
-        workspace = torch.empty(_workspace_bytes(device, entry.matrices, entry.rows, entry.cols, n_rows),
-                                dtype=torch.uint8, device=x.device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         rc = self._lib.nz_mx4_linear(
-            _ptr(entry.packed), entry.matrices, entry.rows, entry.cols,
-            _DTYPES[x.dtype], _ptr(x), x.stride(0), n_rows, per_input, _ptr(ids), _ptr(bias), _ptr(y),
-            _ptr(workspace), workspace.numel(), _ptr(self._status_of(device)), self._use(entry))
+            entry.packed.data_ptr(), entry.matrices, entry.rows, entry.cols, _DTYPES[x.dtype], x.data_ptr(),
+            x.stride(0), n_rows, per_input, _ptr(ids), _ptr(bias), y.data_ptr(), _ptr(workspace), need,
+            self._status_of(device).data_ptr(), self._use(entry))
         if rc:
             _lib.check(rc)
 

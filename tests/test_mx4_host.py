@@ -156,13 +156,14 @@ def test_library_refuses_bad_arguments():
     assert L.nz_mx4_gather_rows(16, 1, 1, 1, 0, 0, 1, 16, 0, 0) == _lib.NZ_E_ARG
     # product: stored bytes, matrices, rows, cols, dtype, x, stride, n_rows, per_input, experts, bias,
     # y, workspace, bytes, status, stream
-    good = [16, 1, 8, 64, 0, 16, 64, 4, 1, 0, 0, 16, 256, 1 << 30, 16, 0]
+    good = [16, 1, 8, 64, 0, 16, 64, 40, 1, 0, 0, 16, 256, 1 << 30, 16, 0]
     for at, value in ((0, 0), (0, 8), (2, 1 << 31), (4, 3), (5, 0), (5, 1), (6, 63), (8, 0), (8, 3), (1, 2),
-                      (11, 0), (12, 0), (12, 16), (7, 1 << 31), (10, 1), (9, 4)):
+                      (11, 0), (12, 16), (7, 1 << 31), (10, 1), (9, 4)):
         bad = list(good)
         bad[at] = value
         assert L.nz_mx4_linear(*bad) == _lib.NZ_E_ARG, (at, value)
-    bad = list(good)
-    bad[13] = 0
-    assert L.nz_mx4_linear(*bad) == _lib.NZ_E_CAPACITY
+    for at in (12, 13):
+        bad = list(good)
+        bad[at] = 0
+        assert L.nz_mx4_linear(*bad) == _lib.NZ_E_CAPACITY
     assert L.nz_mx4_linear(*([0, 0, 8, 64] + [0] * 12)) == _lib.NZ_OK      # no rows: nothing to do
