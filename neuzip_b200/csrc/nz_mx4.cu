@@ -96,10 +96,15 @@ mx4_dequantize_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64
     const uint64_t left = s.cols - (uint64_t)block * kMxBlock;
     uint32_t v[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 f = mx_decode2((c[i / 4] >> (8 * (i & 3))) & 255u);
-      T e[2] = {from_float<T>(f.x * scale), from_float<T>(f.y * scale)};
-      memcpy(&v[i], e, 4);
+    for (int k = 0; k < 4; ++k) {
+      uint32_t pair[4];
+      mx_decode8(c[k], pair);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = mx_unpack2<__half>(pair[i]);
+        T e[2] = {from_float<T>(f.x * scale), from_float<T>(f.y * scale)};
+        memcpy(&v[4 * k + i], e, 4);
+      }
     }
     if (WIDE == 2) {
 #pragma unroll

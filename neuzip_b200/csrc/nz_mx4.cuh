@@ -108,6 +108,18 @@ bool mx_few_rows(const MxShape &w, uint64_t n_rows, bool grouped);
 int mx_few(const MxShape &w, int dtype, const void *packed, const void *x, uint64_t x_stride, uint64_t n_rows,
            uint64_t per_input, const void *experts, const void *bias, void *y, void *status, cudaStream_t st);
 
+// The eight numbers of a word of codes as four pairs of fp16, which holds them exactly.
+__device__ __forceinline__ void mx_decode8(uint32_t word, uint32_t (&pair)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(pair[0]), "=r"(pair[1]), "=r"(pair[2]), "=r"(pair[3])
+      : "r"(word));
+}
+
 // Offset of the scale of row r (in a tile of up to 128 * chunks rows), block b of the step.
 __host__ __device__ __forceinline__ uint32_t mx_scale_offset(uint32_t r, uint32_t b, uint32_t chunks) {
   return ((b >> 2) * chunks + (r >> 7)) * kMxChunk + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (b & 3u);

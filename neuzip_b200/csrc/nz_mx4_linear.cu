@@ -45,6 +45,7 @@ struct MxLinearArgs {
   uint32_t row_tiles, steps, blocks;
   uint32_t x_step_bytes;      // a step of a slot: codes, scales
   uint32_t split;             // 1: the steps of a tile may be shared between CTAs
+  uint32_t in_block;          // stack: few rows of y, which every block groups by itself
   uint32_t stages, stage_bytes;
   uint32_t wide_y;            // 1: rows of y are whole 16-byte pieces
   // workspace
@@ -54,7 +55,7 @@ struct MxLinearArgs {
   uint32_t *row_of;           // stack: row of y at every place of the slots
   uint32_t *place_of;         // stack: place of every row of y, kMxNone without a matrix
   uint8_t *x_packed;
-  float *partial;             // split: a piece [tok][128] of every CTA
+  float *partial;             // split: two pieces [tok][128] of every CTA
 };
 
 // ------------------------------------------------------------------ PTX
@@ -116,6 +117,18 @@ __device__ __forceinline__ bool mx_wait(uint32_t bar, uint32_t parity, const vol
     if ((it & 63u) == 63u && *abort_flag) return false;
   }
   return false;
+}
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mx_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 // The same for a converged warp: one verdict for all lanes.
 __device__ __forceinline__ bool mx_wait_warp(uint32_t bar, uint32_t parity, const volatile uint32_t *abort_flag) {
@@ -227,16 +240,121 @@ __global__ void __launch_bounds__(kMxRouteThreads) mx4_route_kernel(const MxLine
   }
 }
 
+// ------------------------------------------------------------------ few rows, in every block
+// Up to 1024 rows of y and 256 matrices: the blocks of both kernels work the order out for
+// themselves, so that no kernel has to run before them and the product's first copies wait for
+// nothing.  Slots follow the matrices' numbers, places within a matrix the rows' numbers.
+constexpr uint32_t kMxBlockRows = 1024, kMxBlockExperts = 256;
+constexpr uint32_t kMxBlockSlots = kMxBlockExperts + kMxBlockRows / 16;
+
+__device__ __forceinline__ uint32_t mx_expert(const MxLinearArgs &p, uint32_t r) {
+  const int64_t e = r < p.n_rows ? __ldg(p.experts + r) : -1;
+  return e >= 0 && e < (int64_t)p.w.matrices ? (uint32_t)e : kMxNone;
+}
+// The first slot of matrix e = the lane's, of 32 consecutive ones, and the slots up to here.
+__device__ __forceinline__ uint32_t mx_first_slot(uint32_t mine, uint32_t &before) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+    if (lane >= (uint32_t)o) sum += v;
+  }
+  const uint32_t first = before + sum - mine;
+  before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+  return first;
+}
+
+// Places of all rows (256 threads).
+struct MxPlaces {
+  uint16_t count[kMxBlockRows / 32][kMxBlockExperts];      // of 32 rows; then, of the rows before them
+  uint32_t first[kMxBlockExperts];                         // first place of a matrix
+  uint32_t place[kMxBlockRows];
+};
+__device__ __forceinline__ void mx_find_places(const MxLinearArgs &p, MxPlaces &s) {
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t chunks = (p.n_rows + 31) / 32, experts = (uint32_t)p.w.matrices;
+  uint32_t e[4], rank[4];
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) e[i] = mx_expert(p, (warp + 8 * i) * 32 + lane);
+  for (uint32_t i = tid; i < chunks * kMxBlockExperts / 2; i += 256) reinterpret_cast<uint32_t *>(s.count)[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, e[i]);
+    rank[i] = __popc(same & ((1u << lane) - 1u));
+    if (rank[i] == 0 && e[i] != kMxNone) s.count[warp + 8 * i][e[i]] = (uint16_t)__popc(same);
+  }
+  __syncthreads();
+  if (tid < experts) {
+    uint32_t rows = 0;
+    for (uint32_t c = 0; c < chunks; ++c) {
+      const uint32_t here = s.count[c][tid];
+      s.count[c][tid] = (uint16_t)rows;
+      rows += here;
+    }
+    s.first[tid] = (rows + p.tok - 1) / p.tok;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t before = 0;
+    for (uint32_t e0 = 0; e0 < experts; e0 += 32) {
+      const uint32_t first = mx_first_slot(e0 + lane < experts ? s.first[e0 + lane] : 0, before);
+      if (e0 + lane < experts) s.first[e0 + lane] = first * p.tok;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    const uint32_t r = (warp + 8 * i) * 32 + lane;
+    if (r >= p.n_rows) continue;
+    uint32_t place = kMxNone;
+    if (e[i] != kMxNone) {
+      place = s.first[e[i]] + s.count[warp + 8 * i][e[i]] + rank[i];
+      if (blockIdx.x == 0) p.row_of[place] = r;
+    } else if (blockIdx.x == 0 && p.status && __ldg(p.experts + r) != -1) {
+      atomicOr(p.status, NZ_STATUS_BAD_INDEX);
+    }
+    s.place[r] = place;
+  }
+  __syncthreads();
+}
+// The slots alone: matrix << 16 | rows of each, and their number (all threads of the block).
+__device__ __forceinline__ void mx_find_slots(const MxLinearArgs &p, uint32_t *table, uint32_t *count, uint32_t *n) {
+  const uint32_t lane = threadIdx.x & 31, experts = (uint32_t)p.w.matrices;
+  uint32_t e[(kMxBlockRows + kMxLinThreads - 1) / kMxLinThreads];
+#pragma unroll
+  for (uint32_t i = 0; i < sizeof(e) / 4; ++i) e[i] = mx_expert(p, threadIdx.x + i * kMxLinThreads);
+  for (uint32_t i = threadIdx.x; i < experts; i += kMxLinThreads) count[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < sizeof(e) / 4; ++i)
+    if (e[i] != kMxNone) atomicAdd(count + e[i], 1u);
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    uint32_t before = 0;
+    for (uint32_t e0 = 0; e0 < experts; e0 += 32) {
+      const uint32_t rows = e0 + lane < experts ? count[e0 + lane] : 0, mine = (rows + p.tok - 1) / p.tok;
+      const uint32_t first = mx_first_slot(mine, before);
+      for (uint32_t k = 0; k < mine; ++k) table[first + k] = (e0 + lane) << 16 | min(p.tok, rows - k * p.tok);
+    }
+    if (lane == 0) *n = before;
+  }
+  __syncthreads();
+}
+
 // ------------------------------------------------------------------ the rows of x
 // As in mx4_quantize_kernel a thread takes a block, a warp eight rows of x of four blocks.  A row is
 // quantised once and written to the place of every row of y it serves.  Rows of y without a matrix
 // are set to zero here.
 template <typename T, int WIDE>
 __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearArgs p) {
-  if (p.experts) dependent_wait();
+  __shared__ MxPlaces places;
+  if (p.experts && !p.in_block) dependent_wait();
   dependent_trigger();
   const uint32_t lane = threadIdx.x & 31;
-  if (p.split && !p.experts)
+  if (p.in_block) mx_find_places(p, places);
+  if (p.split && (!p.experts || p.in_block))
     for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < p.slots * p.row_tiles; i += gridDim.x * 256)
       p.counters[i] = 0;
   const uint32_t halves = 2 * p.steps, inputs = p.n_rows / p.per_input;
@@ -252,7 +370,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
     if (row >= inputs) continue;
     for (uint32_t j = 0; j < p.per_input; ++j) {
       const uint32_t r = row * p.per_input + j;
-      const uint32_t place = p.experts ? p.place_of[r] : r;
+      const uint32_t place = p.in_block ? places.place[r] : p.experts ? p.place_of[r] : r;
       if (place == kMxNone) {
         // the row's lanes of all its warps share it out
         const uint64_t n = p.w.rows;
@@ -270,40 +388,58 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
 }
 
 // ------------------------------------------------------------------ the product
-// The items of a CTA, in the same order for every role of it.  Where there are at least two CTAs
-// for every tile, its steps are divided among `pieces` of them; else a CTA takes every
-// gridDim.x-th tile.  What an item needs from the slot tables is fetched an item ahead.
+// The items of a CTA, in the same order for every role of it.  A CTA takes every gridDim.x-th tile;
+// or, with p.split, an equal share of all steps of all tiles, one after the other, so that only its
+// first and its last tile are shared with its neighbours (where there are two CTAs or more for a
+// tile, the shares are equal parts of tiles).  What an item needs from the slot tables is fetched an
+// item ahead.
 struct MxItem {
-  uint32_t slot, row_tile, tile, piece, k0, k1, expert, rows;
+  uint32_t slot, row_tile, tile, k0, k1, expert, rows;
 };
 struct MxItems {
   const MxLinearArgs &p;
-  uint32_t n_slots, tiles, pieces;
-  uint32_t at;                // number of the item that is fetched
+  const uint32_t *table;      // slots that the block has worked out
+  uint32_t n_slots, tiles;
+  uint32_t shares;            // split: CTAs that have one
+  uint32_t at, end;           // next tile, or next and last step
   MxItem ahead;
 
-  __device__ __forceinline__ MxItems(const MxLinearArgs &p_, uint32_t n_slots_)
-      : p(p_), n_slots(n_slots_), tiles(n_slots_ * p_.row_tiles), pieces(1), at(blockIdx.x) {
-    if (p.split && tiles) {
-      const uint32_t most = gridDim.x / tiles;
-      pieces = most < 1 ? 1 : most < p.steps ? most : p.steps;
+  __device__ __forceinline__ MxItems(const MxLinearArgs &p_, const uint32_t *table_, uint32_t n_slots_)
+      : p(p_), table(table_), n_slots(n_slots_), tiles(n_slots_ * p_.row_tiles), shares(0), at(blockIdx.x),
+        end(tiles) {
+    if (p.split) {
+      const uint32_t units = tiles * p.steps;
+      shares = gridDim.x;
+      if (tiles && 2 * tiles <= gridDim.x) shares = tiles * min(gridDim.x / tiles, p.steps);
+      if (shares > units) shares = units;
+      at = end = 0;
+      if (blockIdx.x < shares) {
+        at = units * blockIdx.x / shares;          // the plan keeps these products below 2^32
+        end = units * (blockIdx.x + 1) / shares;
+      }
     }
     fetch();
+  }
+  // the CTA whose share has this step: every share has one at least
+  __device__ __forceinline__ uint32_t owner(uint32_t step) const {
+    return ((step + 1) * shares - 1) / (tiles * p.steps);
   }
   // Neighbouring tiles share a tile of W with up to 8 slots, and those slots with the next tiles
   // of W, so that what runs at a time reads little from outside L2.
   __device__ __forceinline__ void fetch() {
-    if (at >= tiles * pieces) return;
-    const uint32_t t = at / pieces;
+    if (at >= end) return;
+    const uint32_t t = p.split ? at / p.steps : at;
     ahead.tile = t;
-    ahead.piece = at - t * pieces;
-    ahead.k0 = p.steps * ahead.piece / pieces;
-    ahead.k1 = p.steps * (ahead.piece + 1) / pieces;
+    ahead.k0 = p.split ? at - t * p.steps : 0;
+    ahead.k1 = p.split ? min(p.steps, ahead.k0 + (end - at)) : p.steps;
     const uint32_t band = t / (8 * p.row_tiles), rest = t - band * 8 * p.row_tiles;
     const uint32_t wide = n_slots - band * 8 < 8 ? n_slots - band * 8 : 8;
     ahead.row_tile = rest / wide;
     ahead.slot = band * 8 + rest - ahead.row_tile * wide;
-    if (p.experts) {
+    if (p.in_block) {
+      ahead.expert = table[ahead.slot] >> 16;
+      ahead.rows = table[ahead.slot] & 0xFFFFu;
+    } else if (p.experts) {
       ahead.expert = __ldcg(p.slot_expert + ahead.slot);
       ahead.rows = __ldcg(p.slot_rows + ahead.slot);
     } else {
@@ -312,12 +448,12 @@ struct MxItems {
     }
   }
   __device__ __forceinline__ bool next(MxItem &item) {
-    if (at >= tiles * pieces) return false;
+    if (at >= end) return false;
     item = ahead;
     // the same in all lanes; the shuffle lets the compiler know
     item.expert = __shfl_sync(0xFFFFFFFFu, item.expert, 0);
     item.rows = __shfl_sync(0xFFFFFFFFu, item.rows, 0);
-    at += gridDim.x;
+    at += p.split ? item.k1 - item.k0 : gridDim.x;
     fetch();
     return true;
   }
@@ -327,9 +463,9 @@ struct MxItems {
 constexpr uint32_t kMxBarFull = 0, kMxBarEmpty = 8 * kMxMaxStages, kMxBarAccFull = 16 * kMxMaxStages,
                    kMxBarAccEmpty = kMxBarAccFull + 16, kMxBarDrain = kMxBarAccEmpty + 16,
                    kMxTmemSlot = kMxBarDrain + 8,
-                   kMxAbortSlot = kMxTmemSlot + 4, kMxLastSlot = kMxAbortSlot + 4, kMxTurn = 256,
-                   kMxMiscBytes = kMxTurn + 4 * 1024;      // 16 rows x 32 features of y for each storing warp
-static_assert(kMxLastSlot + 4 <= kMxTurn, "barriers");
+                   kMxAbortSlot = kMxTmemSlot + 4, kMxLastSlot = kMxAbortSlot + 4, kMxSlotCount = kMxLastSlot + 4, kMxTurn = 256,
+                   kMxTable = kMxTurn + 4 * 1024, kMxMiscBytes = kMxTable + 4 * kMxBlockSlots;      // 16 rows x 32 features of y for each storing warp
+static_assert(kMxSlotCount + 4 <= kMxTurn && 4 * kMxBlockExperts <= 4 * 1024, "barriers");
 
 template <typename T>
 __global__ void __launch_bounds__(kMxLinThreads, 1)
@@ -356,20 +492,52 @@ mx4_product_kernel(const MxLinearArgs p) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  dependent_wait();
-  // after the wait: a CTA that holds tensor memory never waits for another kernel
+  // The allocation may wait for another kernel's CTA on this SM to free its columns; that CTA never
+  // waits for this one, nor does the kernel that this one waits for below, which uses none.
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                      misc_a + kMxTmemSlot)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  uint32_t *table = reinterpret_cast<uint32_t *>(misc + kMxTable);
+  if (p.in_block)
+    mx_find_slots(p, table, reinterpret_cast<uint32_t *>(misc + kMxTurn),
+                  reinterpret_cast<uint32_t *>(misc + kMxSlotCount));
   mx_fence_before();
   __syncthreads();
   mx_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t *>(misc + kMxTmemSlot), 0);
-  const uint32_t n_slots = p.experts ? __shfl_sync(0xFFFFFFFFu, __ldcg(p.n_slots), 0) : p.slots;
-  MxItems items(p, n_slots);
+  // W does not come from the kernel before, which is this call's own: the first stages' are on their
+  // way while that kernel runs, unless the items depend on its tables.
+  const bool known = !p.experts || p.in_block;
+  auto slots_now = [&]() {
+    return !p.experts ? p.slots
+           : p.in_block ? __shfl_sync(0xFFFFFFFFu, *reinterpret_cast<uint32_t *>(misc + kMxSlotCount), 0)
+                        : __shfl_sync(0xFFFFFFFFu, __ldcg(p.n_slots), 0);
+  };
+  auto w_tile = [&](const MxItem &it) {
+    return p.packed + ((uint64_t)it.expert * p.row_tiles + it.row_tile) * p.tile_bytes;
+  };
+  auto w_step_bytes = [&](uint32_t k) { return min(8u, p.blocks - 8 * k) * kMxBlockBytes + 2 * kMxChunk; };
+  uint32_t early = 0;
+  if (warp == 0 && known) {
+    MxItems items(p, table, slots_now());
+    MxItem it;
+    while (early < p.stages && items.next(it)) {
+      const uint8_t *w = w_tile(it) + (uint64_t)it.k0 * kMxStepBytes;
+      for (uint32_t k = it.k0; k < it.k1 && early < p.stages; ++k, ++early, w += kMxStepBytes) {
+        const uint32_t bar = misc_a + kMxBarFull + 8 * early, bytes = w_step_bytes(k);
+        if (mx_elect()) {
+          mbar_expect_tx(bar, bytes + p.x_step_bytes);
+          bulk_g2s(base + early * p.stage_bytes, w, bytes, bar);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  dependent_wait();
+  MxItems items(p, table, slots_now());
 
   if (warp == 0) {
     // ---------------------------------------------------------------- copies
@@ -378,19 +546,21 @@ mx4_product_kernel(const MxLinearArgs p) {
     bool ok = true;
     MxItem it;
     while (ok && items.next(it)) {
-      const uint8_t *w = p.packed + ((uint64_t)it.expert * p.row_tiles + it.row_tile) * p.tile_bytes;
-      const uint8_t *x = p.x_packed + (uint64_t)it.slot * p.steps * p.x_step_bytes;
-      for (uint32_t k = it.k0; k < it.k1; ++k, ++done) {
+      const uint8_t *x = p.x_packed + ((uint64_t)it.slot * p.steps + it.k0) * p.x_step_bytes;
+      const uint8_t *w = w_tile(it) + (uint64_t)it.k0 * kMxStepBytes;
+      for (uint32_t k = it.k0; k < it.k1; ++k, ++done, w += kMxStepBytes, x += p.x_step_bytes) {
         if (done >= p.stages && !mx_wait_warp(misc_a + kMxBarEmpty + 8 * stage, phase ^ 1, abort_flag)) {
           ok = false;
           break;
         }
         const uint32_t at = base + stage * p.stage_bytes, bar = misc_a + kMxBarFull + 8 * stage;
-        const uint32_t w_bytes = min(8u, p.blocks - 8 * k) * kMxBlockBytes + 2 * kMxChunk;
+        const uint32_t bytes = w_step_bytes(k);
         if (mx_elect()) {
-          mbar_expect_tx(bar, w_bytes + p.x_step_bytes);
-          bulk_g2s(at, w + (uint64_t)k * kMxStepBytes, w_bytes, bar);
-          bulk_g2s(at + kMxStepBytes, x + (uint64_t)k * p.x_step_bytes, p.x_step_bytes, bar);
+          if (done >= early) {
+            mbar_expect_tx(bar, bytes + p.x_step_bytes);
+            bulk_g2s(at, w, bytes, bar);
+          }
+          bulk_g2s(at + kMxStepBytes, x, p.x_step_bytes, bar);
         }
         __syncwarp();
         if (++stage == p.stages) {
@@ -415,6 +585,10 @@ mx4_product_kernel(const MxLinearArgs p) {
     uint32_t stage = 0, phase = 0, item = 0;
     bool ok = true;
     const uint32_t k64 = (p.blocks + 1) / 2;
+    const uint64_t a_step = 2 * kMxTileRows, b_step = 2 * p.tok;       // two blocks, in descriptor units
+    // whether the next step is there is asked before this one's products are issued: the answer
+    // takes a hundred cycles
+    bool there = mx_test(misc_a + kMxBarFull, 0);
     MxItem it;
     while (ok && items.next(it)) {
       const uint32_t n = (it.rows + 15u) & ~15u;
@@ -425,14 +599,19 @@ mx4_product_kernel(const MxLinearArgs p) {
         ok = false;
         break;
       }
-      mx_fence_after();
       for (uint32_t k = it.k0; k < it.k1; ++k) {
-        if (!mx_wait_warp(misc_a + kMxBarFull + 8 * stage, phase, abort_flag)) {
+        const uint32_t at = base + stage * p.stage_bytes, empty = misc_a + kMxBarEmpty + 8 * stage;
+        if (!__all_sync(0xFFFFFFFFu, there) &&
+            !mx_wait_warp(misc_a + kMxBarFull + 8 * stage, phase, abort_flag)) {
           ok = false;
           break;
         }
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+        there = mx_test(misc_a + kMxBarFull + 8 * stage, phase);
         mx_fence_after();
-        const uint32_t at = base + stage * p.stage_bytes;
         const uint64_t ad = mx_desc_codes(at, kMxTileRows), bd = mx_desc_codes(at + kMxStepBytes, p.tok);
         const uint64_t sfa = mx_desc_scales(at + min(8u, p.blocks - 8 * k) * kMxBlockBytes);
         const uint64_t sfb = mx_desc_scales(at + kMxStepBytes + 128 * p.tok);
@@ -452,17 +631,13 @@ mx4_product_kernel(const MxLinearArgs p) {
             // product's start at byte 2
             constexpr uint32_t kSecond = (2u << 4) | (2u << 29);
             if (j < last)
-              mx_mma(d, ad + 2 * j * kMxTileRows, bd + 2 * j * p.tok, idesc0 | ((j & 1u) ? kSecond : 0u),
+              mx_mma(d, ad + j * a_step, bd + j * b_step, idesc0 | ((j & 1u) ? kSecond : 0u),
                      tmem + kMxSfA + 4 * (j >> 1), tmem + kMxSfB + 8 * (j >> 1), (k > it.k0) | (j > 0));
           }
-          mx_commit(misc_a + kMxBarEmpty + 8 * stage);
+          mx_commit(empty);
           if (k + 1 == it.k1) mx_commit(misc_a + kMxBarAccFull + 8 * acc);
         }
         __syncwarp();
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
       ++item;
     }
@@ -524,8 +699,12 @@ mx4_product_kernel(const MxLinearArgs p) {
         break;
       }
       mx_fence_after();
-      const bool whole = items.pieces == 1;
-      float *piece = whole ? nullptr : p.partial + (uint64_t)blockIdx.x * p.tok * kMxTileRows + 32 * sub + lane;
+      const bool whole = it.k0 == 0 && it.k1 == p.steps;
+      // pieces of a CTA: its first tile's where it does not begin it, and its last one's
+      auto piece_of = [&](uint32_t cta, bool begins) {
+        return p.partial + ((uint64_t)cta * 2 + begins) * p.tok * kMxTileRows + 32 * sub + lane;
+      };
+      float *piece = whole ? nullptr : piece_of(blockIdx.x, it.k0 == 0);
       for (uint32_t c0 = 0; c0 < rows; c0 += 16) {
         uint32_t v[16];
         mx_tmem_ld16(d + c0, v);
@@ -551,27 +730,29 @@ mx4_product_kernel(const MxLinearArgs p) {
       }
       if (!whole) {
         // The CTA that brings the last piece of a tile adds all of them, in the order of the steps.
+        const uint32_t first = items.owner(it.tile * p.steps);
+        const uint32_t pieces = items.owner(it.tile * p.steps + p.steps - 1) - first + 1;
         __threadfence();
         mx_store_barrier();
         if (threadIdx.x == 64) {
           const uint32_t seen = atomicAdd(p.counters + it.tile, 1u);
           __threadfence();
-          *last_flag = seen == items.pieces - 1;
+          *last_flag = seen == pieces - 1;
         }
         mx_store_barrier();
         if (*last_flag) {
-          const float *from = p.partial + (uint64_t)it.tile * items.pieces * p.tok * kMxTileRows + 32 * sub + lane;
           for (uint32_t c0 = 0; c0 < rows; c0 += 16) {
             float sum[16] = {};
             const uint32_t row_here = row_at(c0);
-            for (uint32_t q0 = 0; q0 < items.pieces; q0 += 4) {
+            for (uint32_t q0 = 0; q0 < pieces; q0 += 4) {
               float add[4][16];                       // loads in flight
 #pragma unroll
               for (uint32_t q = 0; q < 4; ++q)
 #pragma unroll
                 for (uint32_t i = 0; i < 16; ++i)
-                  add[q][i] = q0 + q < items.pieces && c0 + i < rows
-                                  ? __ldcg(from + ((uint64_t)(q0 + q) * p.tok + c0 + i) * kMxTileRows) : 0.f;
+                  add[q][i] = q0 + q < pieces && c0 + i < rows
+                                  ? __ldcg(piece_of(first + q0 + q, q0 + q == 0) + (uint64_t)(c0 + i) * kMxTileRows)
+                                  : 0.f;
 #pragma unroll
               for (uint32_t q = 0; q < 4; ++q)
 #pragma unroll
@@ -597,46 +778,56 @@ mx4_product_kernel(const MxLinearArgs p) {
 
 // --------------------------------------------------------------------- host
 struct MxPlan {
-  uint32_t tok, chunks, row_tiles, steps, split, grid, stages, stage_bytes, x_step_bytes;
+  uint32_t tok, chunks, row_tiles, steps, split, in_block, grid, stages, stage_bytes, x_step_bytes;
   uint64_t slots;
   uint64_t counters, slot_expert, slot_rows, row_of, place_of, x_packed, partial, bytes;
 };
 
-// The rows of a slot, by an estimate of the time (in cycles) that the product takes with them: an
-// SM takes in about 40 bytes a cycle, the tensor cores need 2 cycles a row and step, and what
-// an item costs beside its steps grows with its rows.
-static double mx_cost(uint64_t tok, double slots, uint64_t row_tiles, uint64_t steps, uint32_t sms) {
-  const double tiles = slots * (double)row_tiles;
-  double pieces = 1, waves = ceil(tiles / sms);
-  if (tiles * 2 <= sms) {
-    pieces = floor(sms / tiles);
-    if (pieces > (double)steps) pieces = (double)steps;
-    waves = 1;
+// The rows of a slot, and whether tiles are shared, by an estimate of the time (in cycles) that the
+// product takes: an SM takes in some 60 bytes a cycle, all of them together 3400 from memory, the
+// tensor cores need 2 cycles a row and step, what an item costs beside its steps and what joining
+// pieces costs grow with its rows.
+static double mx_cost(uint64_t tok, double slots, const MxShape &w, double hit, uint32_t sms, bool split) {
+  const double tiles = slots * (double)w.row_tiles(), steps = (double)w.steps();
+  const double load = (kMxStepBytes + tok * 128.0 + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 60.0;
+  const double mma = 2.0 * tok, step = load > mma ? load : mma;
+  const double memory = hit * (double)(w.row_tiles() * w.tile_bytes()) / 3400.0;
+  double steps_in_turn = ceil(tiles / sms) * steps, join = 0;
+  if (split) {
+    double shares = sms;
+    if (2 * tiles <= sms) shares = tiles * fmin(floor(sms / tiles), steps);
+    steps_in_turn = ceil(tiles * steps / shares);
+    join = 2500 + 40.0 * tok;
   }
-  const double load = (kMxStepBytes + tok * 128.0 + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 40.0;
-  const double mma = 2.0 * tok;
-  const double step = load > mma ? load : mma;
-  return waves * (ceil(steps / pieces) * step + 1000 + 8.0 * tok) +
-         (pieces > 1 ? 2000 + 4.0 * tok * pieces : 0);
+  const double product = steps_in_turn * step + ceil(tiles / sms) * 300;
+  return (product > memory ? product : memory) + join + 8.0 * tok;
 }
 
 static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) {
   const uint32_t sms = (uint32_t)sm_count();
   g.row_tiles = (uint32_t)w.row_tiles();
   g.steps = (uint32_t)w.steps();
+  g.in_block = grouped && n_rows <= kMxBlockRows && w.matrices <= kMxBlockExperts;
   const uint64_t groups = grouped ? (w.matrices < n_rows ? w.matrices : n_rows) : 1;
   // matrices that are likely to be named, and half a slot of each that stays empty
   const double hit = grouped ? (double)w.matrices * (1 - pow(1 - 1.0 / (double)w.matrices, (double)n_rows)) : 1;
   uint64_t tok = 16;
-  double best = 0;
+  double best = -1;
+  g.split = 0;
   for (uint64_t t = 16; t <= kMxMaxTok; t += 16) {
     double slots = grouped ? (double)n_rows / t + hit / 2 : ceil((double)n_rows / t);
     if (slots < hit) slots = hit;
-    const double cost = mx_cost(t, slots, g.row_tiles, g.steps, sms);
-    if (t == 16 || cost < best) {
-      best = cost;
-      tok = t;
+    for (int split = 0; split < 2; ++split) {
+      // steps times CTAs in 32 bits, and no more than a few tiles a CTA, or nothing is gained
+      if (split && (g.steps == 1 || slots * (double)w.row_tiles() * g.steps > 4e6)) continue;
+      const double cost = mx_cost(t, slots, w, hit, sms, split != 0);
+      if (best < 0 || cost < best) {
+        best = cost;
+        tok = t;
+        g.split = split;
+      }
     }
+    if (t >= n_rows) break;
   }
   g.tok = (uint32_t)tok;
   g.chunks = g.tok > 128 ? 2 : 1;
@@ -644,8 +835,7 @@ static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) 
   g.slots = grouped ? (n_rows - groups) / tok + groups : (n_rows + tok - 1) / tok;
   const uint64_t tiles = g.slots * g.row_tiles;
   if (g.slots * tok >= (1ull << 31) || tiles >= (1ull << 31)) return false;
-  // a stack may turn out to need fewer tiles than there can be
-  g.split = g.steps > 1 && (grouped ? tiles < 2ull * sms : 2 * tiles <= sms);
+  if (g.split && tiles * g.steps >= (1ull << 32) / (sms + 1)) g.split = 0;
   const uint64_t units = g.split ? tiles * g.steps : tiles;
   g.grid = (uint32_t)(units < sms ? units : sms);
   g.x_step_bytes = g.tok * 128 + g.chunks * 2 * kMxChunk;
@@ -658,13 +848,14 @@ static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) 
     at += (bytes + 255) & ~255ull;
     return here;
   };
+  const bool tables = grouped && !g.in_block;
   g.counters = take(g.split ? tiles * 4 : 0);
-  g.slot_expert = take(grouped ? g.slots * 4 : 0);
-  g.slot_rows = take(grouped ? g.slots * 4 : 0);
+  g.slot_expert = take(tables ? g.slots * 4 : 0);
+  g.slot_rows = take(tables ? g.slots * 4 : 0);
   g.row_of = take(grouped ? g.slots * tok * 4 : 0);
-  g.place_of = take(grouped ? n_rows * 4 : 0);
+  g.place_of = take(tables ? n_rows * 4 : 0);
   g.x_packed = take(g.slots * g.steps * g.x_step_bytes);
-  g.partial = take(g.split ? (uint64_t)g.grid * tok * kMxTileRows * 4 : 0);
+  g.partial = take(g.split ? (uint64_t)g.grid * 2 * tok * kMxTileRows * 4 : 0);
   g.bytes = at;
   return true;
 }
@@ -694,7 +885,7 @@ static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
   auto rows_kernel = wide == 2   ? mx4_quantize_rows_kernel<T, 2>
                      : wide == 1 ? mx4_quantize_rows_kernel<T, 1>
                                  : mx4_quantize_rows_kernel<T, 0>;
-  if (p.experts) {
+  if (p.experts && !p.in_block) {
     NZ_CUDA_TRY(mx_opt_in(mx4_route_kernel, (int)(kMxMaxExperts * 8), route_done));
     mx4_route_kernel<<<1, kMxRouteThreads, p.w.matrices * 8, st>>>(p);
     NZ_LAUNCH_CHECK("mx4_route_kernel");
@@ -792,6 +983,7 @@ extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t row
   p.blocks = (uint32_t)w.blocks();
   p.x_step_bytes = g.x_step_bytes;
   p.split = g.split;
+  p.in_block = g.in_block;
   p.stages = g.stages;
   p.stage_bytes = g.stage_bytes;
   p.wide_y = rows % 8 == 0 && ((uintptr_t)y & 15) == 0;
