@@ -118,22 +118,6 @@ __device__ __forceinline__ bool mx_wait(uint32_t bar, uint32_t parity, const vol
   }
   return false;
 }
-// Whether the phase has completed, without waiting.
-__device__ __forceinline__ bool mx_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// The same for a converged warp: one verdict for all lanes.
-__device__ __forceinline__ bool mx_wait_warp(uint32_t bar, uint32_t parity, const volatile uint32_t *abort_flag) {
-  return __all_sync(0xFFFFFFFFu, mx_wait(bar, parity, abort_flag));
-}
 // One lane of a converged warp.  The instructions below take their operands from the registers that
 // a warp shares; a branch that the compiler knows to be one lane's leaves the operands there, while
 // under `lane == 0` every one is moved across first (a step of four products took 1000 cycles to
@@ -450,9 +434,6 @@ struct MxItems {
   __device__ __forceinline__ bool next(MxItem &item) {
     if (at >= end) return false;
     item = ahead;
-    // the same in all lanes; the shuffle lets the compiler know
-    item.expert = __shfl_sync(0xFFFFFFFFu, item.expert, 0);
-    item.rows = __shfl_sync(0xFFFFFFFFu, item.rows, 0);
     at += p.split ? item.k1 - item.k0 : gridDim.x;
     fetch();
     return true;
@@ -513,110 +494,97 @@ mx4_product_kernel(const MxLinearArgs p) {
   const bool known = !p.experts || p.in_block;
   auto slots_now = [&]() {
     return !p.experts ? p.slots
-           : p.in_block ? __shfl_sync(0xFFFFFFFFu, *reinterpret_cast<uint32_t *>(misc + kMxSlotCount), 0)
-                        : __shfl_sync(0xFFFFFFFFu, __ldcg(p.n_slots), 0);
+           : p.in_block ? *reinterpret_cast<uint32_t *>(misc + kMxSlotCount) : __ldcg(p.n_slots);
   };
   auto w_tile = [&](const MxItem &it) {
     return p.packed + ((uint64_t)it.expert * p.row_tiles + it.row_tile) * p.tile_bytes;
   };
   auto w_step_bytes = [&](uint32_t k) { return min(8u, p.blocks - 8 * k) * kMxBlockBytes + 2 * kMxChunk; };
-  uint32_t early = 0;
-  if (warp == 0 && known) {
-    MxItems items(p, table, slots_now());
-    MxItem it;
-    while (early < p.stages && items.next(it)) {
-      const uint8_t *w = w_tile(it) + (uint64_t)it.k0 * kMxStepBytes;
-      for (uint32_t k = it.k0; k < it.k1 && early < p.stages; ++k, ++early, w += kMxStepBytes) {
-        const uint32_t bar = misc_a + kMxBarFull + 8 * early, bytes = w_step_bytes(k);
-        if (mx_elect()) {
-          mbar_expect_tx(bar, bytes + p.x_step_bytes);
-          bulk_g2s(base + early * p.stage_bytes, w, bytes, bar);
-        }
-      }
-    }
-    __syncwarp();
-  }
-  dependent_wait();
-  MxItems items(p, table, slots_now());
-
   if (warp == 0) {
     // ---------------------------------------------------------------- copies
-    uint32_t stage = 0, phase = 0;
-    uint64_t done = 0;
-    bool ok = true;
-    MxItem it;
-    while (ok && items.next(it)) {
-      const uint8_t *x = p.x_packed + ((uint64_t)it.slot * p.steps + it.k0) * p.x_step_bytes;
-      const uint8_t *w = w_tile(it) + (uint64_t)it.k0 * kMxStepBytes;
-      for (uint32_t k = it.k0; k < it.k1; ++k, ++done, w += kMxStepBytes, x += p.x_step_bytes) {
-        if (done >= p.stages && !mx_wait_warp(misc_a + kMxBarEmpty + 8 * stage, phase ^ 1, abort_flag)) {
-          ok = false;
-          break;
+    if (mx_elect()) {
+      uint32_t early = 0;
+      if (known) {
+        MxItems items(p, table, slots_now());
+        MxItem it;
+        while (early < p.stages && items.next(it)) {
+          const uint8_t *w = w_tile(it) + (uint64_t)it.k0 * kMxStepBytes;
+          for (uint32_t k = it.k0; k < it.k1 && early < p.stages; ++k, ++early, w += kMxStepBytes) {
+            const uint32_t bar = misc_a + kMxBarFull + 8 * early, bytes = w_step_bytes(k);
+            mbar_expect_tx(bar, bytes + p.x_step_bytes);
+            bulk_g2s(base + early * p.stage_bytes, w, bytes, bar);
+          }
         }
-        const uint32_t at = base + stage * p.stage_bytes, bar = misc_a + kMxBarFull + 8 * stage;
-        const uint32_t bytes = w_step_bytes(k);
-        if (mx_elect()) {
+      }
+      dependent_wait();
+      uint32_t stage = 0, phase = 0;
+      uint64_t done = 0;
+      bool ok = true;
+      MxItems items(p, table, slots_now());
+      MxItem it;
+      while (ok && items.next(it)) {
+        const uint8_t *x = p.x_packed + ((uint64_t)it.slot * p.steps + it.k0) * p.x_step_bytes;
+        const uint8_t *w = w_tile(it) + (uint64_t)it.k0 * kMxStepBytes;
+        for (uint32_t k = it.k0; k < it.k1; ++k, ++done, w += kMxStepBytes, x += p.x_step_bytes) {
+          if (done >= p.stages && !mx_wait(misc_a + kMxBarEmpty + 8 * stage, phase ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t at = base + stage * p.stage_bytes, bar = misc_a + kMxBarFull + 8 * stage;
           if (done >= early) {
+            const uint32_t bytes = w_step_bytes(k);
             mbar_expect_tx(bar, bytes + p.x_step_bytes);
             bulk_g2s(at, w, bytes, bar);
           }
           bulk_g2s(at + kMxStepBytes, x, p.x_step_bytes, bar);
-        }
-        __syncwarp();
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1;
+          if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
       }
-    }
-    if (!ok) {
-      if (lane == 0 && p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
-      *abort_flag = 1;
-      // copies still in flight land before the CTA's shared memory is given away: after an abort
-      // nobody else waits for them
-      for (uint64_t i = done > p.stages ? done - p.stages : 0; i < done; ++i) {
-        const uint32_t s = (uint32_t)(i % p.stages), ph = (uint32_t)(i / p.stages) & 1u;
-        for (uint32_t n = 0; n < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarFull + 8 * s, ph); ++n) {
+      if (!ok) {
+        if (p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
+        *abort_flag = 1;
+        // copies still in flight land before the CTA's shared memory is given away: after an abort
+        // nobody else waits for them
+        for (uint64_t i = done > p.stages ? done - p.stages : 0; i < done; ++i) {
+          const uint32_t s = (uint32_t)(i % p.stages), ph = (uint32_t)(i / p.stages) & 1u;
+          for (uint32_t n = 0; n < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarFull + 8 * s, ph); ++n) {
+          }
         }
       }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- tensor cores
-    uint32_t stage = 0, phase = 0, item = 0;
-    bool ok = true;
-    const uint32_t k64 = (p.blocks + 1) / 2;
-    const uint64_t a_step = 2 * kMxTileRows, b_step = 2 * p.tok;       // two blocks, in descriptor units
-    // whether the next step is there is asked before this one's products are issued: the answer
-    // takes a hundred cycles
-    bool there = mx_test(misc_a + kMxBarFull, 0);
-    MxItem it;
-    while (ok && items.next(it)) {
-      const uint32_t n = (it.rows + 15u) & ~15u;
-      // 4-bit operands (type 1), e8m0 scales, M = 128
-      const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | (1u << 27);
-      const uint32_t acc = item & 1u, d = tmem + (acc ? kMxAcc1 : 0u);
-      if (item >= 2 && !mx_wait_warp(misc_a + kMxBarAccEmpty + 8 * acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) {
-        ok = false;
-        break;
-      }
-      for (uint32_t k = it.k0; k < it.k1; ++k) {
-        const uint32_t at = base + stage * p.stage_bytes, empty = misc_a + kMxBarEmpty + 8 * stage;
-        if (!__all_sync(0xFFFFFFFFu, there) &&
-            !mx_wait_warp(misc_a + kMxBarFull + 8 * stage, phase, abort_flag)) {
+    dependent_wait();
+    if (mx_elect()) {
+      uint32_t stage = 0, phase = 0, item = 0;
+      bool ok = true;
+      const uint32_t k64 = (p.blocks + 1) / 2;
+      const uint64_t a_step = 2 * kMxTileRows, b_step = 2 * p.tok;       // two blocks, in descriptor units
+      MxItems items(p, table, slots_now());
+      MxItem it;
+      while (ok && items.next(it)) {
+        const uint32_t n = (it.rows + 15u) & ~15u;
+        // 4-bit operands (type 1), e8m0 scales, M = 128
+        const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | (1u << 27);
+        const uint32_t acc = item & 1u, d = tmem + (acc ? kMxAcc1 : 0u);
+        if (item >= 2 && !mx_wait(misc_a + kMxBarAccEmpty + 8 * acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) {
           ok = false;
           break;
         }
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1;
-        }
-        there = mx_test(misc_a + kMxBarFull + 8 * stage, phase);
-        mx_fence_after();
-        const uint64_t ad = mx_desc_codes(at, kMxTileRows), bd = mx_desc_codes(at + kMxStepBytes, p.tok);
-        const uint64_t sfa = mx_desc_scales(at + min(8u, p.blocks - 8 * k) * kMxBlockBytes);
-        const uint64_t sfb = mx_desc_scales(at + kMxStepBytes + 128 * p.tok);
-        const uint32_t last = min(4u, k64 - 4 * k);
-        if (mx_elect()) {
+        for (uint32_t k = it.k0; k < it.k1; ++k) {
+          const uint32_t at = base + stage * p.stage_bytes;
+          if (!mx_wait(misc_a + kMxBarFull + 8 * stage, phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          mx_fence_after();
+          const uint64_t ad = mx_desc_codes(at, kMxTileRows), bd = mx_desc_codes(at + kMxStepBytes, p.tok);
+          const uint64_t sfa = mx_desc_scales(at + min(8u, p.blocks - 8 * k) * kMxBlockBytes);
+          const uint64_t sfb = mx_desc_scales(at + kMxStepBytes + 128 * p.tok);
+          const uint32_t last = min(4u, k64 - 4 * k);
           // copies and products of one thread run in order: the scales of the step before have
           // been used when these replace them
 #pragma unroll
@@ -634,24 +602,28 @@ mx4_product_kernel(const MxLinearArgs p) {
               mx_mma(d, ad + j * a_step, bd + j * b_step, idesc0 | ((j & 1u) ? kSecond : 0u),
                      tmem + kMxSfA + 4 * (j >> 1), tmem + kMxSfB + 8 * (j >> 1), (k > it.k0) | (j > 0));
           }
-          mx_commit(empty);
-          if (k + 1 == it.k1) mx_commit(misc_a + kMxBarAccFull + 8 * acc);
+          mx_commit(misc_a + kMxBarEmpty + 8 * stage);
+          if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
-        __syncwarp();
+        if (ok) mx_commit(misc_a + kMxBarAccFull + 8 * acc);
+        ++item;
       }
-      ++item;
-    }
-    if (!ok) {
-      if (lane == 0 && p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
-      *abort_flag = 1;
-      // what has been issued still uses shared and tensor memory
-      if (mx_elect()) mx_commit(misc_a + kMxBarDrain);
-      __syncwarp();
-      for (uint32_t n = 0; n < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarDrain, 0); ++n) {
+      if (!ok) {
+        if (p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
+        *abort_flag = 1;
+        // what has been issued still uses shared and tensor memory
+        mx_commit(misc_a + kMxBarDrain);
+        for (uint32_t n = 0; n < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarDrain, 0); ++n) {
+        }
       }
     }
   } else {
     // ---------------------------------------------------------------- results
+    dependent_wait();
+    MxItems items(p, table, slots_now());
     const uint32_t sub = warp & 3u;                   // tensor-memory lanes 32 sub .. + 31
     T *turn = reinterpret_cast<T *>(misc + kMxTurn) + sub * 512;
     uint32_t item = 0;
@@ -784,23 +756,24 @@ struct MxPlan {
 };
 
 // The rows of a slot, and whether tiles are shared, by an estimate of the time (in cycles) that the
-// product takes: an SM takes in some 60 bytes a cycle, all of them together 3400 from memory, the
-// tensor cores need 2 cycles a row and step, what an item costs beside its steps and what joining
-// pieces costs grow with its rows.
+// product takes: an SM takes in some 50 bytes a cycle beside its products, all of them together 3400
+// from memory, the tensor cores need 2 cycles a row and step; what an item costs beside its steps and
+// what joining pieces costs grow with its rows.
 static double mx_cost(uint64_t tok, double slots, const MxShape &w, double hit, uint32_t sms, bool split) {
   const double tiles = slots * (double)w.row_tiles(), steps = (double)w.steps();
-  const double load = (kMxStepBytes + tok * 128.0 + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 60.0;
-  const double mma = 2.0 * tok, step = load > mma ? load : mma;
-  const double memory = hit * (double)(w.row_tiles() * w.tile_bytes()) / 3400.0;
-  double steps_in_turn = ceil(tiles / sms) * steps, join = 0;
+  const double load = (kMxStepBytes + tok * 128.0 + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 50.0;
+  const double mma = 2.0 * tok, busy = load > mma ? load : mma;
+  // a step's share of what comes from memory, with so many tiles at work: slots of a matrix share it
+  auto step = [&](double active) {
+    const double memory = kMxStepBytes * (hit / slots) * active / 3400.0;
+    return busy > memory ? busy : memory;
+  };
   if (split) {
-    double shares = sms;
-    if (2 * tiles <= sms) shares = tiles * fmin(floor(sms / tiles), steps);
-    steps_in_turn = ceil(tiles * steps / shares);
-    join = 2500 + 40.0 * tok;
+    const double shares = 2 * tiles <= sms ? tiles * fmin(floor(sms / tiles), steps) : sms;
+    return ceil(tiles * steps / shares) * step(shares) + 3000 + 50.0 * tok;
   }
-  const double product = steps_in_turn * step + ceil(tiles / sms) * 300;
-  return (product > memory ? product : memory) + join + 8.0 * tok;
+  const double waves = floor(tiles / sms), rest = tiles - waves * sms;
+  return waves * (steps * step(sms) + 300) + (rest > 0 ? steps * step(rest) + 300 : 0) + 8.0 * tok;
 }
 
 static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) {
