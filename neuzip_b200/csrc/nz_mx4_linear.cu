@@ -8,6 +8,7 @@
 //   quantise   turns the rows of x into codes and scales, in slot order, in the workspace
 //   product    one work item = (slot, tile of 128 rows of W, range of steps of 256 columns)
 // A tile of W is the M side of the MMA (128 tensor-memory lanes), a slot the N side (its columns).
+#include <cuda.h>
 #include <math.h>
 #include <string.h>
 
@@ -46,6 +47,7 @@ struct MxLinearArgs {
   uint32_t x_step_bytes;      // a step of a slot: codes, scales
   uint32_t split;             // 1: the steps of a tile may be shared between CTAs
   uint32_t in_block;          // stack: few rows of y, which every block groups by itself
+  uint32_t pair;              // 1: two CTAs share a slot's step and take two tiles of W
   uint32_t stages, stage_bytes;
   uint32_t wide_y;            // 1: rows of y are whole 16-byte pieces
   // workspace
@@ -78,24 +80,89 @@ __device__ __forceinline__ uint64_t mx_desc_codes(uint32_t addr, uint32_t rows) 
 __device__ __forceinline__ uint64_t mx_desc_scales(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | (8ull << 32) | (1ull << 46);
 }
+// The instructions of a CTA alone and of a pair of CTAs (PAIR: issued by the pair's first CTA, they
+// use both CTAs' shared and tensor memory at the same addresses).
 // One chunk of scales (32 rows of 16 bytes) to four tensor-memory columns, the same in all four
 // groups of 32 lanes.
+template <bool PAIR>
 __device__ __forceinline__ void mx_copy_scales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  if (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 // D (+)= A B^T over 64 columns, a scale per 32 columns of either operand.
+template <bool PAIR>
 __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
                                        uint32_t sfb, uint32_t accumulate) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// Arrives at the barrier (of both CTAs of a pair) when what this thread has issued is done.
+template <bool PAIR>
+__device__ __forceinline__ void mx_commit(uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+                 : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void mx_tmem_alloc(uint32_t slot) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void mx_tmem_free(uint32_t tmem) {
+  if (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+// This CTA's number in its pair; an arrival at the first CTA's barrier; a barrier of both CTAs.
+__device__ __forceinline__ uint32_t mx_pair_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t mx_of_first(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void mx_arrive_first(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mx_of_first(bar)) : "memory");
+}
+// A run of 256-byte rows to this CTA's shared memory; its bytes count at a barrier of either CTA of the
+// pair, which only the tensor form of the copy can do.
+__device__ __forceinline__ void mx_pair_copy(uint32_t dst, const CUtensorMap *map, int32_t row, uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(0), "r"(row)
       : "memory");
 }
-__device__ __forceinline__ void mx_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-               : "memory");
+__device__ __forceinline__ void mx_pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void mx_tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
@@ -114,6 +181,22 @@ __device__ __forceinline__ void mx_tmem_ld_wait() {
 __device__ __forceinline__ bool mx_wait(uint32_t bar, uint32_t parity, const volatile uint32_t *abort_flag) {
   for (uint32_t it = 0; it < kMaxWaitIters; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 63u && *abort_flag) return false;
+  }
+  return false;
+}
+// The same on a barrier at which the other CTA of a pair arrives.
+__device__ __forceinline__ bool mx_wait_pair(uint32_t bar, uint32_t parity, const volatile uint32_t *abort_flag) {
+  for (uint32_t it = 0; it < kMaxWaitIters; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kWaitHintNs)
+        : "memory");
+    if (ok) return true;
     if ((it & 63u) == 63u && *abort_flag) return false;
   }
   return false;
@@ -327,6 +410,9 @@ __device__ __forceinline__ void mx_find_slots(const MxLinearArgs &p, uint32_t *t
   __syncthreads();
 }
 
+// Columns of a product for so many rows of x.
+__device__ __forceinline__ uint32_t mx_columns(uint32_t rows) { return (rows + 15u) & ~15u; }
+
 // ------------------------------------------------------------------ the rows of x
 // As in mx4_quantize_kernel a thread takes a block, a warp eight rows of x of four blocks.  A row is
 // quantised once and written to the place of every row of y it serves.  Rows of y without a matrix
@@ -363,8 +449,14 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
       }
       const uint32_t slot = place / p.tok, i = place - slot * p.tok;
       uint8_t *step = p.x_packed + ((uint64_t)slot * p.steps + (half >> 1)) * p.x_step_bytes;
-      *reinterpret_cast<uint4 *>(step + ((block & 7u) * p.tok + i) * 16) =
-          make_uint4(code[0], code[1], code[2], code[3]);
+      uint32_t at = (block & 7u) * p.tok + i;
+      if (p.pair) {
+        // the first half of the product's columns, then the second, each on its own
+        const uint32_t rows = p.experts ? __ldcg(p.slot_rows + slot) : min(p.tok, p.n_rows - slot * p.tok);
+        const uint32_t split = mx_columns(rows) / 2, second = i >= split;
+        at = (8 * second + (block & 7u)) * (p.tok / 2) + i - second * split;
+      }
+      *reinterpret_cast<uint4 *>(step + at * 16) = make_uint4(code[0], code[1], code[2], code[3]);
       if (lane < 8)
         *reinterpret_cast<uint32_t *>(step + 128 * p.tok + mx_scale_offset(i, (half & 1) * 4, p.chunks)) = word;
     }
@@ -375,7 +467,8 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
 // The items of a CTA, in the same order for every role of it.  A CTA takes every gridDim.x-th tile;
 // or, with p.split, an equal share of all steps of all tiles, one after the other, so that only its
 // first and its last tile are shared with its neighbours (where there are two CTAs or more for a
-// tile, the shares are equal parts of tiles).  What an item needs from the slot tables is fetched an
+// tile, the shares are equal parts of tiles).  For a pair of CTAs (p.pair, never with p.split) a tile is
+// two tiles of W, one for each.  What an item needs from the slot tables is fetched an
 // item ahead.
 struct MxItem {
   uint32_t slot, row_tile, tile, k0, k1, expert, rows;
@@ -383,14 +476,15 @@ struct MxItem {
 struct MxItems {
   const MxLinearArgs &p;
   const uint32_t *table;      // slots that the block has worked out
-  uint32_t n_slots, tiles;
+  uint32_t n_slots, tiles, across;     // across: tiles that a slot has
   uint32_t shares;            // split: CTAs that have one
   uint32_t at, end;           // next tile, or next and last step
   MxItem ahead;
 
   __device__ __forceinline__ MxItems(const MxLinearArgs &p_, const uint32_t *table_, uint32_t n_slots_)
-      : p(p_), table(table_), n_slots(n_slots_), tiles(n_slots_ * p_.row_tiles), shares(0), at(blockIdx.x),
-        end(tiles) {
+      : p(p_), table(table_), n_slots(n_slots_), across(p_.pair ? (p_.row_tiles + 1) / 2 : p_.row_tiles),
+        shares(0), at(p_.pair ? blockIdx.x / 2 : blockIdx.x) {
+    tiles = end = n_slots * across;
     if (p.split) {
       const uint32_t units = tiles * p.steps;
       shares = gridDim.x;
@@ -416,7 +510,7 @@ struct MxItems {
     ahead.tile = t;
     ahead.k0 = p.split ? at - t * p.steps : 0;
     ahead.k1 = p.split ? min(p.steps, ahead.k0 + (end - at)) : p.steps;
-    const uint32_t band = t / (8 * p.row_tiles), rest = t - band * 8 * p.row_tiles;
+    const uint32_t band = t / (8 * across), rest = t - band * 8 * across;
     const uint32_t wide = n_slots - band * 8 < 8 ? n_slots - band * 8 : 8;
     ahead.row_tile = rest / wide;
     ahead.slot = band * 8 + rest - ahead.row_tile * wide;
@@ -434,10 +528,15 @@ struct MxItems {
   __device__ __forceinline__ bool next(MxItem &item) {
     if (at >= end) return false;
     item = ahead;
-    at += p.split ? item.k1 - item.k0 : gridDim.x;
+    at += p.split ? item.k1 - item.k0 : p.pair ? gridDim.x / 2 : gridDim.x;
     fetch();
     return true;
   }
+};
+
+// Pair: W, the codes of a pair's half of a slot's step, and its scales, as rows of 256 bytes.
+struct MxPairMaps {
+  CUtensorMap w, x_codes, x_scales;
 };
 
 // Shared-memory map: stages (a step of a tile of W, a step of a slot), then
@@ -448,9 +547,9 @@ constexpr uint32_t kMxBarFull = 0, kMxBarEmpty = 8 * kMxMaxStages, kMxBarAccFull
                    kMxTable = kMxTurn + 4 * 1024, kMxMiscBytes = kMxTable + 4 * kMxBlockSlots;      // 16 rows x 32 features of y for each storing warp
 static_assert(kMxSlotCount + 4 <= kMxTurn && 4 * kMxBlockExperts <= 4 * 1024, "barriers");
 
-template <typename T>
+template <typename T, bool PAIR>
 __global__ void __launch_bounds__(kMxLinThreads, 1)
-mx4_product_kernel(const MxLinearArgs p) {
+mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps) {
   extern __shared__ uint8_t mx_smem[];
   const uint32_t base = (smem_u32(mx_smem) + 127u) & ~127u;
   const uint32_t misc_a = base + p.stages * p.stage_bytes;
@@ -467,7 +566,7 @@ mx4_product_kernel(const MxLinearArgs p) {
     }
     for (uint32_t a = 0; a < 2; ++a) {
       mbar_init(misc_a + kMxBarAccFull + 8 * a, 1);
-      mbar_init(misc_a + kMxBarAccEmpty + 8 * a, 4);
+      mbar_init(misc_a + kMxBarAccEmpty + 8 * a, PAIR ? 8 : 4);      // storing warps
     }
     mbar_init(misc_a + kMxBarDrain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -476,10 +575,7 @@ mx4_product_kernel(const MxLinearArgs p) {
   // The allocation may wait for another kernel's CTA on this SM to free its columns; that CTA never
   // waits for this one, nor does the kernel that this one waits for below, which uses none.
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
-                     misc_a + kMxTmemSlot)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    mx_tmem_alloc<PAIR>(misc_a + kMxTmemSlot);
   }
   uint32_t *table = reinterpret_cast<uint32_t *>(misc + kMxTable);
   if (p.in_block)
@@ -487,7 +583,9 @@ mx4_product_kernel(const MxLinearArgs p) {
                   reinterpret_cast<uint32_t *>(misc + kMxSlotCount));
   mx_fence_before();
   __syncthreads();
+  if (PAIR) mx_pair_sync();                    // both CTAs' barriers are there
   mx_fence_after();
+  const uint32_t rank = PAIR ? mx_pair_rank() : 0;
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t *>(misc + kMxTmemSlot), 0);
   // W does not come from the kernel before, which is this call's own: the first stages' are on their
   // way while that kernel runs, unless the items depend on its tables.
@@ -496,24 +594,48 @@ mx4_product_kernel(const MxLinearArgs p) {
     return !p.experts ? p.slots
            : p.in_block ? *reinterpret_cast<uint32_t *>(misc + kMxSlotCount) : __ldcg(p.n_slots);
   };
+  // the CTA's tile of W; where a pair has one tile left, the second CTA reads it too and stores nothing
+  auto my_tile = [&](const MxItem &it) { return PAIR ? 2 * it.row_tile + rank : it.row_tile; };
   auto w_tile = [&](const MxItem &it) {
-    return p.packed + ((uint64_t)it.expert * p.row_tiles + it.row_tile) * p.tile_bytes;
+    return p.packed + ((uint64_t)it.expert * p.row_tiles + min(my_tile(it), p.row_tiles - 1)) * p.tile_bytes;
   };
-  auto w_step_bytes = [&](uint32_t k) { return min(8u, p.blocks - 8 * k) * kMxBlockBytes + 2 * kMxChunk; };
+  const uint32_t x_rows = PAIR ? p.tok / 2 : p.tok;                 // rows of a slot that this CTA holds
+  const uint32_t x_codes = x_rows * 128, x_scales = p.chunks * 2 * kMxChunk, x_bytes = x_codes + x_scales;
   if (warp == 0) {
     // ---------------------------------------------------------------- copies
     if (mx_elect()) {
+      // the bytes of a stage count at this CTA's barrier; a pair's at the first CTA's, which expects
+      // the second one's too.  A pair copies whole steps (behind a tile's short last step lies the next
+      // tile, or zeros).
+      auto load_w = [&](const uint8_t *w, uint32_t k, uint32_t stage) {
+        const uint32_t at = base + stage * p.stage_bytes, bar = misc_a + kMxBarFull + 8 * stage;
+        if (PAIR) {
+          if (rank == 0) mbar_expect_tx(bar, 2 * (kMxStepBytes + x_bytes));
+          mx_pair_copy(at, &maps.w, (int32_t)((w - p.packed) / 256), mx_of_first(bar));
+        } else {
+          const uint32_t bytes = min(8u, p.blocks - 8 * k) * kMxBlockBytes + 2 * kMxChunk;
+          mbar_expect_tx(bar, bytes + x_bytes);
+          bulk_g2s(at, w, bytes, bar);
+        }
+      };
+      auto load_x = [&](const uint8_t *x, uint32_t stage) {
+        const uint32_t at = base + stage * p.stage_bytes + kMxStepBytes, bar = misc_a + kMxBarFull + 8 * stage;
+        if (PAIR) {
+          const int32_t row = (int32_t)((x - p.x_packed) / 256), half = (int32_t)(x_codes / 256);
+          mx_pair_copy(at, &maps.x_codes, row + (int32_t)rank * half, mx_of_first(bar));
+          mx_pair_copy(at + x_codes, &maps.x_scales, row + 2 * half, mx_of_first(bar));
+        } else {
+          bulk_g2s(at, x, x_bytes, bar);
+        }
+      };
       uint32_t early = 0;
       if (known) {
         MxItems items(p, table, slots_now());
         MxItem it;
         while (early < p.stages && items.next(it)) {
           const uint8_t *w = w_tile(it) + (uint64_t)it.k0 * kMxStepBytes;
-          for (uint32_t k = it.k0; k < it.k1 && early < p.stages; ++k, ++early, w += kMxStepBytes) {
-            const uint32_t bar = misc_a + kMxBarFull + 8 * early, bytes = w_step_bytes(k);
-            mbar_expect_tx(bar, bytes + p.x_step_bytes);
-            bulk_g2s(base + early * p.stage_bytes, w, bytes, bar);
-          }
+          for (uint32_t k = it.k0; k < it.k1 && early < p.stages; ++k, ++early, w += kMxStepBytes)
+            load_w(w, k, early);
         }
       }
       dependent_wait();
@@ -530,13 +652,8 @@ mx4_product_kernel(const MxLinearArgs p) {
             ok = false;
             break;
           }
-          const uint32_t at = base + stage * p.stage_bytes, bar = misc_a + kMxBarFull + 8 * stage;
-          if (done >= early) {
-            const uint32_t bytes = w_step_bytes(k);
-            mbar_expect_tx(bar, bytes + p.x_step_bytes);
-            bulk_g2s(at, w, bytes, bar);
-          }
-          bulk_g2s(at + kMxStepBytes, x, p.x_step_bytes, bar);
+          if (done >= early) load_w(w, k, stage);
+          load_x(x, stage);
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
@@ -547,8 +664,8 @@ mx4_product_kernel(const MxLinearArgs p) {
         if (p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
         *abort_flag = 1;
         // copies still in flight land before the CTA's shared memory is given away: after an abort
-        // nobody else waits for them
-        for (uint64_t i = done > p.stages ? done - p.stages : 0; i < done; ++i) {
+        // nobody else waits for them (a pair's first CTA does so for both)
+        for (uint64_t i = done > p.stages ? done - p.stages : 0; i < done && rank == 0; ++i) {
           const uint32_t s = (uint32_t)(i % p.stages), ph = (uint32_t)(i / p.stages) & 1u;
           for (uint32_t n = 0; n < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarFull + 8 * s, ph); ++n) {
           }
@@ -558,19 +675,19 @@ mx4_product_kernel(const MxLinearArgs p) {
   } else if (warp == 1) {
     // ---------------------------------------------------------------- tensor cores
     dependent_wait();
-    if (mx_elect()) {
+    if (rank == 0 && mx_elect()) {
       uint32_t stage = 0, phase = 0, item = 0;
       bool ok = true;
       const uint32_t k64 = (p.blocks + 1) / 2;
-      const uint64_t a_step = 2 * kMxTileRows, b_step = 2 * p.tok;       // two blocks, in descriptor units
+      const uint64_t a_step = 2 * kMxTileRows, b_step = 2 * x_rows;      // two blocks, in descriptor units
       MxItems items(p, table, slots_now());
       MxItem it;
       while (ok && items.next(it)) {
-        const uint32_t n = (it.rows + 15u) & ~15u;
-        // 4-bit operands (type 1), e8m0 scales, M = 128
-        const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | (1u << 27);
+        // 4-bit operands (type 1), e8m0 scales, N, M = 128 or 256
+        const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((mx_columns(it.rows) >> 3) << 17) | (1u << 23) |
+                                ((PAIR ? 2u : 1u) << 27);
         const uint32_t acc = item & 1u, d = tmem + (acc ? kMxAcc1 : 0u);
-        if (item >= 2 && !mx_wait(misc_a + kMxBarAccEmpty + 8 * acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) {
+        if (item >= 2 && !mx_wait_pair(misc_a + kMxBarAccEmpty + 8 * acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) {
           ok = false;
           break;
         }
@@ -581,17 +698,17 @@ mx4_product_kernel(const MxLinearArgs p) {
             break;
           }
           mx_fence_after();
-          const uint64_t ad = mx_desc_codes(at, kMxTileRows), bd = mx_desc_codes(at + kMxStepBytes, p.tok);
+          const uint64_t ad = mx_desc_codes(at, kMxTileRows), bd = mx_desc_codes(at + kMxStepBytes, x_rows);
           const uint64_t sfa = mx_desc_scales(at + min(8u, p.blocks - 8 * k) * kMxBlockBytes);
-          const uint64_t sfb = mx_desc_scales(at + kMxStepBytes + 128 * p.tok);
+          const uint64_t sfb = mx_desc_scales(at + kMxStepBytes + x_codes);
           const uint32_t last = min(4u, k64 - 4 * k);
           // copies and products of one thread run in order: the scales of the step before have
           // been used when these replace them
 #pragma unroll
           for (uint32_t h = 0; h < 2; ++h) {
-            mx_copy_scales(tmem + kMxSfA + 4 * h, sfa + h * (kMxChunk >> 4));
-            mx_copy_scales(tmem + kMxSfB + 8 * h, sfb + h * p.chunks * (kMxChunk >> 4));
-            if (p.chunks == 2) mx_copy_scales(tmem + kMxSfB + 8 * h + 4, sfb + (2 * h + 1) * (kMxChunk >> 4));
+            mx_copy_scales<PAIR>(tmem + kMxSfA + 4 * h, sfa + h * (kMxChunk >> 4));
+            mx_copy_scales<PAIR>(tmem + kMxSfB + 8 * h, sfb + h * p.chunks * (kMxChunk >> 4));
+            if (p.chunks == 2) mx_copy_scales<PAIR>(tmem + kMxSfB + 8 * h + 4, sfb + (2 * h + 1) * (kMxChunk >> 4));
           }
 #pragma unroll
           for (uint32_t j = 0; j < 4; ++j) {
@@ -599,23 +716,23 @@ mx4_product_kernel(const MxLinearArgs p) {
             // product's start at byte 2
             constexpr uint32_t kSecond = (2u << 4) | (2u << 29);
             if (j < last)
-              mx_mma(d, ad + j * a_step, bd + j * b_step, idesc0 | ((j & 1u) ? kSecond : 0u),
+              mx_mma<PAIR>(d, ad + j * a_step, bd + j * b_step, idesc0 | ((j & 1u) ? kSecond : 0u),
                      tmem + kMxSfA + 4 * (j >> 1), tmem + kMxSfB + 8 * (j >> 1), (k > it.k0) | (j > 0));
           }
-          mx_commit(misc_a + kMxBarEmpty + 8 * stage);
+          mx_commit<PAIR>(misc_a + kMxBarEmpty + 8 * stage);
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if (ok) mx_commit(misc_a + kMxBarAccFull + 8 * acc);
+        if (ok) mx_commit<PAIR>(misc_a + kMxBarAccFull + 8 * acc);
         ++item;
       }
       if (!ok) {
         if (p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
         *abort_flag = 1;
         // what has been issued still uses shared and tensor memory
-        mx_commit(misc_a + kMxBarDrain);
+        mx_commit<PAIR>(misc_a + kMxBarDrain);
         for (uint32_t n = 0; n < kMaxWaitIters && !mbar_try_wait(misc_a + kMxBarDrain, 0); ++n) {
         }
       }
@@ -630,18 +747,18 @@ mx4_product_kernel(const MxLinearArgs p) {
     MxItem it;
     while (items.next(it)) {
       const uint32_t rows = it.rows, place0 = it.slot * p.tok;
-      const uint32_t feature = it.row_tile * kMxTileRows + 32 * sub + lane;
+      const uint32_t feature = my_tile(it) * kMxTileRows + 32 * sub + lane;
       const bool real = feature < p.w.rows;
       const float bias = p.bias && real ? to_float<T>(((const T *)p.bias)[it.expert * p.w.rows + feature]) : 0.f;
       // 16 rows of y of this warp's 32 features, from a value for every row in each lane
-      T *y = (T *)p.y + it.row_tile * kMxTileRows + 32 * sub;
+      T *y = (T *)p.y + my_tile(it) * kMxTileRows + 32 * sub;
       auto store16 = [&](const float (&f)[16], uint32_t row_here, uint32_t count) {
         if (p.wide_y) {
           // turned in shared memory: four lanes take a row's 64 bytes
 #pragma unroll
           for (uint32_t i = 0; i < 16; ++i) turn[i * 32 + lane] = from_float<T>(f[i] + bias);
           __syncwarp();
-          const bool in = it.row_tile * kMxTileRows + 32 * sub + 8 * (lane & 3u) < p.w.rows;
+          const bool in = my_tile(it) * kMxTileRows + 32 * sub + 8 * (lane & 3u) < p.w.rows;
 #pragma unroll
           for (uint32_t h = 0; h < 2; ++h) {
             const uint32_t i = 8 * h + (lane >> 2);
@@ -687,7 +804,10 @@ mx4_product_kernel(const MxLinearArgs p) {
           // the last columns are out: the tensor cores may have this accumulator again
           mx_fence_before();
           __syncwarp();
-          if (lane == 0) mx_mbar_arrive(misc_a + kMxBarAccEmpty + 8 * acc);
+          if (lane == 0) {
+            if (PAIR) mx_arrive_first(misc_a + kMxBarAccEmpty + 8 * acc);
+            else mx_mbar_arrive(misc_a + kMxBarAccEmpty + 8 * acc);
+          }
         }
         if (!whole) {
 #pragma unroll
@@ -738,19 +858,21 @@ mx4_product_kernel(const MxLinearArgs p) {
     }
   }
 
-  // ---- common exit: everybody is done with tensor memory, then it is freed
+  // ---- common exit: everybody is done with tensor memory (and with the other CTA's barriers), then
+  // it is freed
   __syncwarp();
   mx_fence_before();
   __syncthreads();
+  if (PAIR) mx_pair_sync();
   if (warp == 1) {
     mx_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    mx_tmem_free<PAIR>(tmem);
   }
 }
 
 // --------------------------------------------------------------------- host
 struct MxPlan {
-  uint32_t tok, chunks, row_tiles, steps, split, in_block, grid, stages, stage_bytes, x_step_bytes;
+  uint32_t tok, chunks, row_tiles, steps, split, in_block, pair, grid, stages, stage_bytes, x_step_bytes;
   uint64_t slots;
   uint64_t counters, slot_expert, slot_rows, row_of, place_of, x_packed, partial, bytes;
 };
@@ -759,16 +881,19 @@ struct MxPlan {
 // product takes: an SM takes in some 50 bytes a cycle beside its products, all of them together 3400
 // from memory, the tensor cores need 2 cycles a row and step; what an item costs beside its steps and
 // what joining pieces costs grow with its rows.
-static double mx_cost(uint64_t tok, double slots, const MxShape &w, double hit, uint32_t sms, bool split) {
-  const double tiles = slots * (double)w.row_tiles(), steps = (double)w.steps();
-  const double load = (kMxStepBytes + tok * 128.0 + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 50.0;
+// `kind`: whole tiles, shared tiles, or tiles of a pair of CTAs, of which `sms` then counts the pairs.
+enum MxKind { kMxWhole, kMxShared, kMxPaired };
+static double mx_cost(uint64_t tok, double slots, const MxShape &w, double hit, uint32_t sms, MxKind kind) {
+  const double pair = kind == kMxPaired ? 2 : 1;
+  const double tiles = slots * ceil((double)w.row_tiles() / pair), steps = (double)w.steps();
+  const double load = (kMxStepBytes + tok * 128.0 / pair + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 50.0;
   const double mma = 2.0 * tok, busy = load > mma ? load : mma;
   // a step's share of what comes from memory, with so many tiles at work: slots of a matrix share it
   auto step = [&](double active) {
-    const double memory = kMxStepBytes * (hit / slots) * active / 3400.0;
+    const double memory = pair * kMxStepBytes * (hit / slots) * active / 3400.0;
     return busy > memory ? busy : memory;
   };
-  if (split) {
+  if (kind == kMxShared) {
     const double shares = 2 * tiles <= sms ? tiles * fmin(floor(sms / tiles), steps) : sms;
     return ceil(tiles * steps / shares) * step(shares) + 3000 + 50.0 * tok;
   }
@@ -776,8 +901,11 @@ static double mx_cost(uint64_t tok, double slots, const MxShape &w, double hit, 
   return waves * (steps * step(sms) + 300) + (rest > 0 ? steps * step(rest) + 300 : 0) + 8.0 * tok;
 }
 
-static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) {
-  const uint32_t sms = (uint32_t)sm_count();
+// Pairs of CTAs that the device runs at a time.
+static uint32_t mx_pairs();
+
+static bool mx_make_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) {
+  const uint32_t sms = (uint32_t)sm_count(), n_pairs = mx_pairs();
   g.row_tiles = (uint32_t)w.row_tiles();
   g.steps = (uint32_t)w.steps();
   g.in_block = grouped && n_rows <= kMxBlockRows && w.matrices <= kMxBlockExperts;
@@ -786,18 +914,21 @@ static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) 
   const double hit = grouped ? (double)w.matrices * (1 - pow(1 - 1.0 / (double)w.matrices, (double)n_rows)) : 1;
   uint64_t tok = 16;
   double best = -1;
-  g.split = 0;
+  g.split = g.pair = 0;
   for (uint64_t t = 16; t <= kMxMaxTok; t += 16) {
     double slots = grouped ? (double)n_rows / t + hit / 2 : ceil((double)n_rows / t);
     if (slots < hit) slots = hit;
-    for (int split = 0; split < 2; ++split) {
+    for (MxKind kind : {kMxWhole, kMxShared, kMxPaired}) {
       // steps times CTAs in 32 bits, and no more than a few tiles a CTA, or nothing is gained
-      if (split && (g.steps == 1 || slots * (double)w.row_tiles() * g.steps > 4e6)) continue;
-      const double cost = mx_cost(t, slots, w, hit, sms, split != 0);
+      if (kind == kMxShared && (g.steps == 1 || slots * (double)w.row_tiles() * g.steps > 4e6)) continue;
+      // the places of a pair's inputs depend on the slots' rows, which tables tell
+      if (kind == kMxPaired && (g.in_block || n_pairs == 0)) continue;
+      const double cost = mx_cost(t, slots, w, hit, kind == kMxPaired ? n_pairs : sms, kind);
       if (best < 0 || cost < best) {
         best = cost;
         tok = t;
-        g.split = split;
+        g.split = kind == kMxShared;
+        g.pair = kind == kMxPaired;
       }
     }
     if (t >= n_rows) break;
@@ -811,8 +942,12 @@ static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) 
   if (g.split && tiles * g.steps >= (1ull << 32) / (sms + 1)) g.split = 0;
   const uint64_t units = g.split ? tiles * g.steps : tiles;
   g.grid = (uint32_t)(units < sms ? units : sms);
+  if (g.pair) {
+    const uint64_t pairs = g.slots * ((g.row_tiles + 1) / 2);
+    g.grid = 2 * (uint32_t)(pairs < n_pairs ? pairs : n_pairs);
+  }
   g.x_step_bytes = g.tok * 128 + g.chunks * 2 * kMxChunk;
-  g.stage_bytes = kMxStepBytes + g.x_step_bytes;
+  g.stage_bytes = kMxStepBytes + (g.pair ? g.tok * 64 + g.chunks * 2 * kMxChunk : g.x_step_bytes);
   g.stages = (kMaxDynamicSmem - 128 - kMxMiscBytes) / g.stage_bytes;
   if (g.stages > kMxMaxStages) g.stages = kMxMaxStages;
   uint64_t at = 256;
@@ -833,24 +968,130 @@ static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) 
   return true;
 }
 
-// The kernel's shared memory above 48 KB has to be asked for once per device.
-template <typename K>
-static cudaError_t mx_opt_in(K kern, int bytes, bool (&done)[kMaxDeviceOrdinals]) {
-  static std::mutex mu;
+// Plans of recent calls: a program makes the same few over and over.
+static bool mx_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan &g) {
+  struct Kept {
+    MxShape w = {0, 0, 0};
+    uint64_t n_rows = 0;
+    int dev = -1;
+    bool grouped = false, fits = false;
+    MxPlan g;
+  };
+  static thread_local Kept kept[64];
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return mx_make_plan(w, n_rows, grouped, g);
+  }
+  Kept &k = kept[(w.rows * 7 + w.cols * 13 + n_rows * 31 + w.matrices * 3 + grouped) % 64];
+  if (k.dev != dev || k.w.matrices != w.matrices || k.w.rows != w.rows || k.w.cols != w.cols ||
+      k.n_rows != n_rows || k.grouped != grouped) {
+    k.fits = mx_make_plan(w, n_rows, grouped, k.g);
+    k.w = w;
+    k.n_rows = n_rows;
+    k.grouped = grouped;
+    k.dev = dev;
+  }
+  g = k.g;
+  return k.fits;
+}
+
+// The kernels' shared memory above 48 KB has to be asked for, and the pairs counted, once per device.
+struct MxDevice {
+  std::mutex mu;
+  bool ready = false;
+  uint32_t pairs = 0;
+};
+static cudaLaunchConfig_t mx_config(unsigned grid, size_t smem, bool pair, cudaStream_t st,
+                                    cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kMxLinThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pair ? 2 : 1;
+  return cfg;
+}
+static cudaError_t mx_device(uint32_t *pairs) {
+  static MxDevice devices[kMaxDeviceOrdinals];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  std::lock_guard<std::mutex> lock(mu);
-  if (dev >= 0 && dev < kMaxDeviceOrdinals && done[dev]) return cudaSuccess;
-  err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (err == cudaSuccess && dev >= 0 && dev < kMaxDeviceOrdinals) done[dev] = true;
-  return err;
+  if (dev < 0 || dev >= kMaxDeviceOrdinals) return cudaErrorInvalidDevice;
+  MxDevice &d = devices[dev];
+  std::lock_guard<std::mutex> lock(d.mu);
+  if (!d.ready) {
+    const int most = (int)kMaxDynamicSmem;
+    const auto larger = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    if ((err = cudaFuncSetAttribute(mx4_product_kernel<__nv_bfloat16, false>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_product_kernel<__half, false>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_product_kernel<__nv_bfloat16, true>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_product_kernel<__half, true>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_route_kernel, larger, (int)(kMxMaxExperts * 8))) != cudaSuccess)
+      return err;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = mx_config(2 * 1024, kMaxDynamicSmem, true, 0, attr);
+    int clusters = 0;
+    if ((err = cudaOccupancyMaxActiveClusters(&clusters, mx4_product_kernel<__nv_bfloat16, true>, &cfg)) !=
+        cudaSuccess)
+      return err;
+    d.pairs = (uint32_t)clusters;
+    d.ready = true;
+  }
+  *pairs = d.pairs;
+  return cudaSuccess;
+}
+static uint32_t mx_pairs() {
+  uint32_t pairs = 0;
+  if (mx_device(&pairs) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;                                  // without a device the size helpers still answer
+  }
+  return pairs;
+}
+
+typedef CUresult (*MxEncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                    CUtensorMapFloatOOBfill);
+static bool mx_map(CUtensorMap *map, const void *bytes, uint64_t rows, uint32_t box) {
+  static std::once_flag once;
+  static MxEncodeTiledFn encode = nullptr;
+  std::call_once(once, [] {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) == cudaSuccess &&
+        found == cudaDriverEntryPointSuccess)
+      encode = (MxEncodeTiledFn)fn;
+  });
+  const cuuint64_t dim[2] = {256, rows}, stride[1] = {256};
+  const cuuint32_t size[2] = {256, box}, step[2] = {1, 1};
+  return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(bytes), dim, stride, size, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T>
 static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
-  static bool product_done[kMaxDeviceOrdinals] = {}, route_done[kMaxDeviceOrdinals] = {};
-  NZ_CUDA_TRY(mx_opt_in(mx4_product_kernel<T>, (int)kMaxDynamicSmem, product_done));
+  MxPairMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  if (p.pair) {
+    const uint64_t x_rows = (uint64_t)p.slots * p.steps * p.x_step_bytes / 256;
+    if (!mx_map(&maps.w, p.packed, p.w.bytes() / 256, kMxStepBytes / 256) ||
+        !mx_map(&maps.x_codes, p.x_packed, x_rows, p.tok / 4) ||
+        !mx_map(&maps.x_scales, p.x_packed, x_rows, p.chunks * 2 * kMxChunk / 256)) {
+      set_error("nz_mx4_linear: cuTensorMapEncodeTiled failed");
+      return NZ_E_CUDA;
+    }
+  }
+  uint32_t pairs = 0;
+  NZ_CUDA_TRY(mx_device(&pairs));
   const int wide = mx_wide_rows(p.x, p.x_stride, p.w.cols);
   const uint64_t warps = (uint64_t)((p.n_rows / p.per_input + 7) / 8) * 2 * p.steps, blocks = (warps + 7) / 8;
   const unsigned most = (unsigned)sm_count() * 8;
@@ -859,7 +1100,6 @@ static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
                      : wide == 1 ? mx4_quantize_rows_kernel<T, 1>
                                  : mx4_quantize_rows_kernel<T, 0>;
   if (p.experts && !p.in_block) {
-    NZ_CUDA_TRY(mx_opt_in(mx4_route_kernel, (int)(kMxMaxExperts * 8), route_done));
     mx4_route_kernel<<<1, kMxRouteThreads, p.w.matrices * 8, st>>>(p);
     NZ_LAUNCH_CHECK("mx4_route_kernel");
     NZ_CUDA_TRY(launch_dependent(rows_kernel, grid, 256, 0, st, p));
@@ -867,8 +1107,11 @@ static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
     rows_kernel<<<grid, 256, 0, st>>>(p);
     NZ_LAUNCH_CHECK("mx4_quantize_rows_kernel");
   }
-  const size_t smem = 128 + (size_t)p.stages * p.stage_bytes + kMxMiscBytes;
-  NZ_CUDA_TRY(launch_dependent(mx4_product_kernel<T>, g.grid, kMxLinThreads, smem, st, p));
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg =
+      mx_config(g.grid, 128 + (size_t)p.stages * p.stage_bytes + kMxMiscBytes, p.pair != 0, st, attr);
+  NZ_CUDA_TRY(p.pair ? cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, true>, p, maps)
+                     : cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, false>, p, maps));
   return NZ_OK;
 }
 
@@ -957,6 +1200,7 @@ extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t row
   p.x_step_bytes = g.x_step_bytes;
   p.split = g.split;
   p.in_block = g.in_block;
+  p.pair = g.pair;
   p.stages = g.stages;
   p.stage_bytes = g.stage_bytes;
   p.wide_y = rows % 8 == 0 && ((uintptr_t)y & 15) == 0;
