@@ -236,6 +236,9 @@ class MX4Manager(Manager):
         self._be = MX4Backend()
         self.meta_dict: Dict[str, torch.Size] = {}
 
+    def linear(self, handle: str, inputs: torch.Tensor, bias=None) -> torch.Tensor:
+        return self._be.linear(handle, inputs, self.meta_dict[handle], bias)
+
     def grouped_linear(self, handle: str, inputs: torch.Tensor, experts: torch.Tensor,
                        bias: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Every row of `inputs` times the matrix that `experts` names for it, for a handle that

@@ -22,7 +22,8 @@ namespace nz {
 
 constexpr uint32_t kMxMaxTok = 240;          // rows of x in a slot: what two accumulators leave room for
 constexpr uint32_t kMxMaxStages = 12;
-constexpr int kMxLinThreads = 192;           // TMA, MMA, 4 warps that store
+constexpr int kMxLinThreads = 192;           // a warp that copies, one that issues, 4 that store
+constexpr uint32_t kMxHelpers = 8;           // fused: more warps that quantise
 constexpr uint32_t kMxMaxExperts = 8192;
 constexpr uint32_t kMxNone = 0xFFFFFFFFu;
 // Tensor memory, 512 columns: two accumulators, between and behind them the scales of one step.
@@ -48,6 +49,8 @@ struct MxLinearArgs {
   uint32_t split;             // 1: the steps of a tile may be shared between CTAs
   uint32_t in_block;          // stack: few rows of y, which every block groups by itself
   uint32_t pair;              // 1: two CTAs share a slot's step and take two tiles of W
+  uint32_t x_resident;        // bytes of a slot's steps in shared memory, quantised there; else 0
+  int wide;                   // how rows of x can be read, see mx_load_block
   uint32_t stages, stage_bytes;
   uint32_t wide_y;            // 1: rows of y are whole 16-byte pieces
   // workspace
@@ -184,6 +187,18 @@ __device__ __forceinline__ bool mx_wait(uint32_t bar, uint32_t parity, const vol
     if ((it & 63u) == 63u && *abort_flag) return false;
   }
   return false;
+}
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mx_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 // The same on a barrier at which the other CTA of a pair arrives.
 __device__ __forceinline__ bool mx_wait_pair(uint32_t bar, uint32_t parity, const volatile uint32_t *abort_flag) {
@@ -386,28 +401,49 @@ __device__ __forceinline__ void mx_find_places(const MxLinearArgs &p, MxPlaces &
   }
   __syncthreads();
 }
-// The slots alone: matrix << 16 | rows of each, and their number (all threads of the block).
-__device__ __forceinline__ void mx_find_slots(const MxLinearArgs &p, uint32_t *table, uint32_t *count, uint32_t *n) {
+// The slots alone (all threads of the block): matrix << 18 | number among the matrix's slots << 9 |
+// rows of each, their number, and the matrix of every row.
+constexpr uint16_t kMxNoMatrix = 0xFFFF;
+template <uint32_t THREADS>
+__device__ __forceinline__ void mx_find_slots(const MxLinearArgs &p, uint32_t *table, uint32_t *count,
+                                              uint16_t *ids, uint32_t *n) {
   const uint32_t lane = threadIdx.x & 31, experts = (uint32_t)p.w.matrices;
-  uint32_t e[(kMxBlockRows + kMxLinThreads - 1) / kMxLinThreads];
+  uint32_t e[(kMxBlockRows + THREADS - 1) / THREADS];
 #pragma unroll
-  for (uint32_t i = 0; i < sizeof(e) / 4; ++i) e[i] = mx_expert(p, threadIdx.x + i * kMxLinThreads);
-  for (uint32_t i = threadIdx.x; i < experts; i += kMxLinThreads) count[i] = 0;
+  for (uint32_t i = 0; i < sizeof(e) / 4; ++i) e[i] = mx_expert(p, threadIdx.x + i * THREADS);
+  for (uint32_t i = threadIdx.x; i < experts; i += THREADS) count[i] = 0;
   __syncthreads();
 #pragma unroll
-  for (uint32_t i = 0; i < sizeof(e) / 4; ++i)
+  for (uint32_t i = 0; i < sizeof(e) / 4; ++i) {
+    const uint32_t r = threadIdx.x + i * THREADS;
+    if (r < kMxBlockRows) ids[r] = (uint16_t)e[i];                 // kMxNone becomes kMxNoMatrix
     if (e[i] != kMxNone) atomicAdd(count + e[i], 1u);
+  }
   __syncthreads();
   if (threadIdx.x < 32) {
     uint32_t before = 0;
     for (uint32_t e0 = 0; e0 < experts; e0 += 32) {
       const uint32_t rows = e0 + lane < experts ? count[e0 + lane] : 0, mine = (rows + p.tok - 1) / p.tok;
       const uint32_t first = mx_first_slot(mine, before);
-      for (uint32_t k = 0; k < mine; ++k) table[first + k] = (e0 + lane) << 16 | min(p.tok, rows - k * p.tok);
+      for (uint32_t k = 0; k < mine; ++k)
+        table[first + k] = (e0 + lane) << 18 | k << 9 | min(p.tok, rows - k * p.tok);
     }
     if (lane == 0) *n = before;
   }
   __syncthreads();
+}
+// The rows of the k-th slot of a matrix, in order (a warp).
+__device__ __forceinline__ void mx_list_rows(const MxLinearArgs &p, const uint16_t *ids, uint32_t matrix, uint32_t k,
+                                             uint16_t *list) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t before = 0;
+  for (uint32_t r0 = 0; r0 < p.n_rows; r0 += 32) {
+    const bool mine = ids[r0 + lane] == matrix;
+    const uint32_t same = __ballot_sync(0xFFFFFFFFu, mine), at = before + __popc(same & ((1u << lane) - 1u)) - k * p.tok;
+    if (mine && at < p.tok) list[at] = (uint16_t)(r0 + lane);
+    before += __popc(same);
+  }
+  __syncwarp();
 }
 
 // Columns of a product for so many rows of x.
@@ -419,27 +455,33 @@ __device__ __forceinline__ uint32_t mx_columns(uint32_t rows) { return (rows + 1
 // are set to zero here.
 template <typename T, int WIDE>
 __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearArgs p) {
-  __shared__ MxPlaces places;
-  if (p.experts && !p.in_block) dependent_wait();
+  extern __shared__ uint32_t rows_smem[];
+  MxPlaces &places = *reinterpret_cast<MxPlaces *>(rows_smem);       // in_block
+  // The product is let in when everything before this kernel is complete, W among it: it begins to
+  // read W while this kernel runs.
+  dependent_wait();
   dependent_trigger();
   const uint32_t lane = threadIdx.x & 31;
   if (p.in_block) mx_find_places(p, places);
   if (p.split && (!p.experts || p.in_block))
     for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < p.slots * p.row_tiles; i += gridDim.x * 256)
       p.counters[i] = 0;
-  const uint32_t halves = 2 * p.steps, inputs = p.n_rows / p.per_input;
+  // Items are rows of x, or where there are few of them rows of y: then a row of x that serves several
+  // is quantised for each, by warps of their own.
+  const uint32_t serves = p.in_block ? 1 : p.per_input, shared = p.per_input / serves;
+  const uint32_t halves = 2 * p.steps, inputs = p.n_rows / serves;
   const uint64_t total = (uint64_t)((inputs + 7) / 8) * halves;
   for (uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (uint64_t)gridDim.x * 8) {
     const uint32_t group = (uint32_t)(w / halves), half = (uint32_t)(w - (uint64_t)group * halves);
     const uint32_t row = group * 8 + (lane & 7u), block = half * 4 + (lane >> 3);
     uint32_t v[16], code[4], byte;
     const int64_t left = row < inputs ? (int64_t)p.w.cols - (int64_t)block * kMxBlock : 0;
-    mx_load_block<WIDE>((const T *)p.x + row * p.x_stride + (uint64_t)block * kMxBlock, left, v);
+    mx_load_block<WIDE>((const T *)p.x + row / shared * p.x_stride + (uint64_t)block * kMxBlock, left, v);
     mx_quantize_block<T>(v, code, byte);
     const uint32_t word = mx_pack_scales(byte, lane);
     if (row >= inputs) continue;
-    for (uint32_t j = 0; j < p.per_input; ++j) {
-      const uint32_t r = row * p.per_input + j;
+    for (uint32_t j = 0; j < serves; ++j) {
+      const uint32_t r = row * serves + j;
       const uint32_t place = p.in_block ? places.place[r] : p.experts ? p.place_of[r] : r;
       if (place == kMxNone) {
         // the row's lanes of all its warps share it out
@@ -471,7 +513,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
 // two tiles of W, one for each.  What an item needs from the slot tables is fetched an
 // item ahead.
 struct MxItem {
-  uint32_t slot, row_tile, tile, k0, k1, expert, rows;
+  uint32_t slot, row_tile, tile, k0, k1, expert, rows, number;
 };
 struct MxItems {
   const MxLinearArgs &p;
@@ -515,8 +557,9 @@ struct MxItems {
     ahead.row_tile = rest / wide;
     ahead.slot = band * 8 + rest - ahead.row_tile * wide;
     if (p.in_block) {
-      ahead.expert = table[ahead.slot] >> 16;
-      ahead.rows = table[ahead.slot] & 0xFFFFu;
+      ahead.expert = table[ahead.slot] >> 18;
+      ahead.number = (table[ahead.slot] >> 9) & 511u;
+      ahead.rows = table[ahead.slot] & 511u;
     } else if (p.experts) {
       ahead.expert = __ldcg(p.slot_expert + ahead.slot);
       ahead.rows = __ldcg(p.slot_rows + ahead.slot);
@@ -539,19 +582,76 @@ struct MxPairMaps {
   CUtensorMap w, x_codes, x_scales;
 };
 
-// Shared-memory map: stages (a step of a tile of W, a step of a slot), then
+// The rows of a slot into shared memory, by all warps that store or help (this one is number `sub`), a
+// block a thread: a warp takes up to 8 rows at a time (as many as a power of two of them that there
+// are) and the blocks of them that fill it, and requests four such pieces before it works on them.
+template <typename T>
+__device__ __forceinline__ void mx_quantize_slot(const MxLinearArgs &p, const MxItem &it, const uint16_t *row_list,
+                                                 uint32_t sub, uint32_t x_at, uint32_t x_codes) {
+  constexpr uint32_t kWarps = 4 + kMxHelpers, kAhead = 4;
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t shift = it.rows > 4 ? 3 : it.rows > 2 ? 2 : it.rows - 1;
+  const uint32_t each = 32u >> shift;                         // blocks of a piece
+  const uint32_t padded = (p.blocks + 1) & ~1u;               // the products take blocks in pairs
+  const uint32_t across = (padded + each - 1) / each, total = ((it.rows - 1) >> shift) + 1;
+  const uint32_t pieces = total * across;
+  for (uint32_t w0 = sub; w0 < pieces; w0 += kWarps * kAhead) {
+    uint32_t v[kAhead][16], to[kAhead], block[kAhead];
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k) {
+      const uint32_t w = w0 + k * kWarps, group = w / across;
+      const uint32_t i = (group << shift) + (lane & ((1u << shift) - 1u));
+      block[k] = (w - group * across) * each + (lane >> shift);
+      const bool there = w < pieces && i < it.rows && block[k] < padded;
+      to[k] = there ? i : kMxNone;
+      const uint32_t row = there ? (p.experts ? row_list[i] : it.slot * p.tok + i) / p.per_input : 0;
+      const T *src = (const T *)p.x + row * p.x_stride + (uint64_t)block[k] * kMxBlock;
+      const int64_t left = there ? (int64_t)p.w.cols - (int64_t)block[k] * kMxBlock : 0;
+      if (p.wide == 2) mx_load_block<2>(src, left, v[k]);
+      else if (p.wide == 1) mx_load_block<1>(src, left, v[k]);
+      else mx_load_block<0>(src, left, v[k]);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k) {
+      if (to[k] == kMxNone) continue;
+      uint32_t code[4], byte;
+      mx_quantize_block<T>(v[k], code, byte);
+      const uint32_t step = x_at + (block[k] >> 3) * p.x_step_bytes;
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(step + ((block[k] & 7u) * p.tok + to[k]) * 16),
+                   "r"(code[0]), "r"(code[1]), "r"(code[2]), "r"(code[3])
+                   : "memory");
+      asm volatile("st.shared.u8 [%0], %1;" ::"r"(step + x_codes + mx_scale_offset(to[k], block[k] & 7u, p.chunks)),
+                   "r"(byte)
+                   : "memory");
+    }
+  }
+  // visible to the tensor cores' reads
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// How a product runs: in CTAs by themselves behind the kernel that quantises x, in pairs of CTAs
+// behind it, or in CTAs that quantise the rows of their slot themselves, in one launch.
+enum MxMode { kMxAlone, kMxPair, kMxFused };
+__host__ __device__ constexpr int mx_threads(MxMode mode) { return kMxLinThreads + (mode == kMxFused ? (int)kMxHelpers * 32 : 0); }
+
+// Shared-memory map: a slot's steps (fused), stages (a step of a tile of W and, unless fused, of a
+// slot), then
 constexpr uint32_t kMxBarFull = 0, kMxBarEmpty = 8 * kMxMaxStages, kMxBarAccFull = 16 * kMxMaxStages,
                    kMxBarAccEmpty = kMxBarAccFull + 16, kMxBarDrain = kMxBarAccEmpty + 16,
-                   kMxTmemSlot = kMxBarDrain + 8,
-                   kMxAbortSlot = kMxTmemSlot + 4, kMxLastSlot = kMxAbortSlot + 4, kMxSlotCount = kMxLastSlot + 4, kMxTurn = 256,
-                   kMxTable = kMxTurn + 4 * 1024, kMxMiscBytes = kMxTable + 4 * kMxBlockSlots;      // 16 rows x 32 features of y for each storing warp
+                   kMxBarX = kMxBarDrain + 8, kMxTmemSlot = kMxBarX + 8, kMxAbortSlot = kMxTmemSlot + 4,
+                   kMxLastSlot = kMxAbortSlot + 4, kMxSlotCount = kMxLastSlot + 4,
+                   kMxTurn = 512,               // 16 rows x 32 features of y for each storing warp
+                   kMxTable = kMxTurn + 4 * 1024, kMxIds = kMxTable + 4 * kMxBlockSlots,
+                   kMxRowList = kMxIds + 2 * kMxBlockRows,      // fused: a slot's rows, for each warp
+                   kMxMiscBytes = kMxRowList + (4 + kMxHelpers) * 512;
 static_assert(kMxSlotCount + 4 <= kMxTurn && 4 * kMxBlockExperts <= 4 * 1024, "barriers");
 
-template <typename T, bool PAIR>
-__global__ void __launch_bounds__(kMxLinThreads, 1)
+template <typename T, MxMode MODE>
+__global__ void __launch_bounds__(mx_threads(MODE), 1)
 mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps) {
+  constexpr bool PAIR = MODE == kMxPair, FUSED = MODE == kMxFused;
   extern __shared__ uint8_t mx_smem[];
-  const uint32_t base = (smem_u32(mx_smem) + 127u) & ~127u;
+  const uint32_t x_at = (smem_u32(mx_smem) + 127u) & ~127u, base = x_at + (FUSED ? p.x_resident : 0);
   const uint32_t misc_a = base + p.stages * p.stage_bytes;
   uint8_t *misc = mx_smem + (misc_a - smem_u32(mx_smem));
   volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(misc + kMxAbortSlot);
@@ -569,17 +669,19 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
       mbar_init(misc_a + kMxBarAccEmpty + 8 * a, PAIR ? 8 : 4);      // storing warps
     }
     mbar_init(misc_a + kMxBarDrain, 1);
+    mbar_init(misc_a + kMxBarX, 4 + kMxHelpers);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  // The allocation may wait for another kernel's CTA on this SM to free its columns; that CTA never
+  // The allocation may wait for a CTA of another kernel on this SM to free its columns; that CTA never
   // waits for this one, nor does the kernel that this one waits for below, which uses none.
   if (warp == 1) {
     mx_tmem_alloc<PAIR>(misc_a + kMxTmemSlot);
   }
   uint32_t *table = reinterpret_cast<uint32_t *>(misc + kMxTable);
+  uint16_t *ids = reinterpret_cast<uint16_t *>(misc + kMxIds);
   if (p.in_block)
-    mx_find_slots(p, table, reinterpret_cast<uint32_t *>(misc + kMxTurn),
+    mx_find_slots<mx_threads(MODE)>(p, table, reinterpret_cast<uint32_t *>(misc + kMxTurn), ids,
                   reinterpret_cast<uint32_t *>(misc + kMxSlotCount));
   mx_fence_before();
   __syncthreads();
@@ -601,6 +703,16 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
   };
   const uint32_t x_rows = PAIR ? p.tok / 2 : p.tok;                 // rows of a slot that this CTA holds
   const uint32_t x_codes = x_rows * 128, x_scales = p.chunks * 2 * kMxChunk, x_bytes = x_codes + x_scales;
+  // fused: a warp's part of an item's rows, unless the item before had the same slot
+  auto prepare_rows = [&](const MxItem &it, uint16_t *row_list, uint32_t sub, uint32_t &have) {
+    if (have != it.slot) {
+      have = it.slot;
+      if (p.in_block) mx_list_rows(p, ids, it.expert, it.number, row_list);
+      mx_quantize_slot<T>(p, it, row_list, sub, x_at, x_codes);
+    }
+    __syncwarp();
+    if (lane == 0) mx_mbar_arrive(misc_a + kMxBarX);
+  };
   if (warp == 0) {
     // ---------------------------------------------------------------- copies
     if (mx_elect()) {
@@ -614,7 +726,7 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
           mx_pair_copy(at, &maps.w, (int32_t)((w - p.packed) / 256), mx_of_first(bar));
         } else {
           const uint32_t bytes = min(8u, p.blocks - 8 * k) * kMxBlockBytes + 2 * kMxChunk;
-          mbar_expect_tx(bar, bytes + x_bytes);
+          mbar_expect_tx(bar, FUSED ? bytes : bytes + x_bytes);
           bulk_g2s(at, w, bytes, bar);
         }
       };
@@ -653,7 +765,7 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
             break;
           }
           if (done >= early) load_w(w, k, stage);
-          load_x(x, stage);
+          if (!FUSED) load_x(x, stage);
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
@@ -679,51 +791,65 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
       uint32_t stage = 0, phase = 0, item = 0;
       bool ok = true;
       const uint32_t k64 = (p.blocks + 1) / 2;
-      const uint64_t a_step = 2 * kMxTileRows, b_step = 2 * x_rows;      // two blocks, in descriptor units
+      // in units of descriptors: two blocks, a stage, the chunks of a step's half
+      const uint64_t a_step = 2 * kMxTileRows, b_step = 2 * x_rows, stage_step = p.stage_bytes >> 4;
+      const uint64_t a_chunk = kMxChunk >> 4, b_chunk = p.chunks * a_chunk;
+      const uint64_t a0 = mx_desc_codes(base, kMxTileRows), sfa0 = mx_desc_scales(base);
+      const uint64_t b0 = mx_desc_codes(FUSED ? x_at : base + kMxStepBytes, x_rows);
+      const uint64_t sfb0 = mx_desc_scales((FUSED ? x_at : base + kMxStepBytes) + x_codes);
+      const bool two = p.chunks == 2;
+      // whether a stage has arrived is asked a step ahead: the answer takes a hundred cycles, which the
+      // issuing of the step before covers
+      bool there = mx_test(misc_a + kMxBarFull, 0);
       MxItems items(p, table, slots_now());
       MxItem it;
       while (ok && items.next(it)) {
         // 4-bit operands (type 1), e8m0 scales, N, M = 128 or 256
         const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((mx_columns(it.rows) >> 3) << 17) | (1u << 23) |
                                 ((PAIR ? 2u : 1u) << 27);
+        const uint32_t idesc1 = idesc0 | (2u << 4) | (2u << 29);       // the scales at byte 2
         const uint32_t acc = item & 1u, d = tmem + (acc ? kMxAcc1 : 0u);
         if (item >= 2 && !mx_wait_pair(misc_a + kMxBarAccEmpty + 8 * acc, ((item >> 1) & 1u) ^ 1u, abort_flag)) {
           ok = false;
           break;
         }
+        if (FUSED && !mx_wait(misc_a + kMxBarX, item & 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
         for (uint32_t k = it.k0; k < it.k1; ++k) {
-          const uint32_t at = base + stage * p.stage_bytes;
-          if (!mx_wait(misc_a + kMxBarFull + 8 * stage, phase, abort_flag)) {
+          if (!there && !mx_wait(misc_a + kMxBarFull + 8 * stage, phase, abort_flag)) {
             ok = false;
             break;
           }
-          mx_fence_after();
-          const uint64_t ad = mx_desc_codes(at, kMxTileRows), bd = mx_desc_codes(at + kMxStepBytes, x_rows);
-          const uint64_t sfa = mx_desc_scales(at + min(8u, p.blocks - 8 * k) * kMxBlockBytes);
-          const uint64_t sfb = mx_desc_scales(at + kMxStepBytes + x_codes);
-          const uint32_t last = min(4u, k64 - 4 * k);
-          // copies and products of one thread run in order: the scales of the step before have
-          // been used when these replace them
-#pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {
-            mx_copy_scales<PAIR>(tmem + kMxSfA + 4 * h, sfa + h * (kMxChunk >> 4));
-            mx_copy_scales<PAIR>(tmem + kMxSfB + 8 * h, sfb + h * p.chunks * (kMxChunk >> 4));
-            if (p.chunks == 2) mx_copy_scales<PAIR>(tmem + kMxSfB + 8 * h + 4, sfb + (2 * h + 1) * (kMxChunk >> 4));
-          }
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) {
-            // 64 columns are two blocks; the scales of four share a tensor-memory column, the second
-            // product's start at byte 2
-            constexpr uint32_t kSecond = (2u << 4) | (2u << 29);
-            if (j < last)
-              mx_mma<PAIR>(d, ad + j * a_step, bd + j * b_step, idesc0 | ((j & 1u) ? kSecond : 0u),
-                     tmem + kMxSfA + 4 * (j >> 1), tmem + kMxSfB + 8 * (j >> 1), (k > it.k0) | (j > 0));
-          }
-          mx_commit<PAIR>(misc_a + kMxBarEmpty + 8 * stage);
+          const uint32_t done = misc_a + kMxBarEmpty + 8 * stage;
+          const uint64_t at = stage * stage_step, x_step = FUSED ? k * (uint64_t)(p.x_step_bytes >> 4) : at;
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
           }
+          there = mx_test(misc_a + kMxBarFull + 8 * stage, phase);
+          mx_fence_after();
+          const uint64_t ad = a0 + at, bd = b0 + x_step, sfb = sfb0 + x_step;
+          const uint64_t sfa = sfa0 + at + min(8u, p.blocks - 8 * k) * (kMxBlockBytes >> 4);
+          const uint32_t last = k64 - 4 * k, more = k > it.k0;
+          // Copies and products of one thread run in order: the scales of the step before have been
+          // used when these replace them.  64 columns are two blocks; the scales of four share a
+          // tensor-memory column.
+          mx_copy_scales<PAIR>(tmem + kMxSfA, sfa);
+          mx_copy_scales<PAIR>(tmem + kMxSfB, sfb);
+          if (two) mx_copy_scales<PAIR>(tmem + kMxSfB + 4, sfb + a_chunk);
+          mx_mma<PAIR>(d, ad, bd, idesc0, tmem + kMxSfA, tmem + kMxSfB, more);
+          if (last > 1) mx_mma<PAIR>(d, ad + a_step, bd + b_step, idesc1, tmem + kMxSfA, tmem + kMxSfB, 1);
+          if (last > 2) {
+            mx_copy_scales<PAIR>(tmem + kMxSfA + 4, sfa + a_chunk);
+            mx_copy_scales<PAIR>(tmem + kMxSfB + 8, sfb + b_chunk);
+            if (two) mx_copy_scales<PAIR>(tmem + kMxSfB + 12, sfb + b_chunk + a_chunk);
+            mx_mma<PAIR>(d, ad + 2 * a_step, bd + 2 * b_step, idesc0, tmem + kMxSfA + 4, tmem + kMxSfB + 8, 1);
+            if (last > 3)
+              mx_mma<PAIR>(d, ad + 3 * a_step, bd + 3 * b_step, idesc1, tmem + kMxSfA + 4, tmem + kMxSfB + 8, 1);
+          }
+          mx_commit<PAIR>(done);
         }
         if (ok) mx_commit<PAIR>(misc_a + kMxBarAccFull + 8 * acc);
         ++item;
@@ -737,15 +863,45 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
         }
       }
     }
+  } else if (FUSED && warp >= 6) {
+    // ---------------------------------------------------------------- rows of x, with the storing warps
+    MxItems items(p, table, slots_now());
+    uint16_t *row_list = reinterpret_cast<uint16_t *>(misc + kMxRowList) + (warp - 2) * 256;
+    uint32_t item = 0, have = kMxNone;
+    MxItem it;
+    while (items.next(it)) {
+      // the slot before has been used when its products are done
+      const uint32_t b = item - 1;
+      if (item && !__all_sync(0xFFFFFFFFu, mx_wait(misc_a + kMxBarAccFull + 8 * (b & 1u), (b >> 1) & 1u, abort_flag))) {
+        if (lane == 0 && p.status) atomicOr(p.status, NZ_STATUS_TIMEOUT);
+        *abort_flag = 1;
+        break;
+      }
+      prepare_rows(it, row_list, warp - 2, have);
+      ++item;
+    }
   } else {
     // ---------------------------------------------------------------- results
     dependent_wait();
     MxItems items(p, table, slots_now());
     const uint32_t sub = warp & 3u;                   // tensor-memory lanes 32 sub .. + 31
     T *turn = reinterpret_cast<T *>(misc + kMxTurn) + sub * 512;
-    uint32_t item = 0;
+    uint16_t *row_list = reinterpret_cast<uint16_t *>(misc + kMxRowList) + sub * 256;
+    if (FUSED && p.in_block) {
+      // rows of y without a matrix
+      for (uint32_t r = blockIdx.x; r < p.n_rows; r += gridDim.x)
+        if (ids[r] == kMxNoMatrix) {
+          for (uint64_t i = 32 * sub + lane; i < p.w.rows; i += 128) ((T *)p.y)[r * p.w.rows + i] = from_float<T>(0.f);
+          if (threadIdx.x == 64 && p.status && __ldg(p.experts + r) != -1) atomicOr(p.status, NZ_STATUS_BAD_INDEX);
+        }
+    }
+    uint32_t item = 0, have = kMxNone;
     MxItem it;
     while (items.next(it)) {
+      if (FUSED) {
+        // the products of the item before are done, or its sums would not have been read
+        prepare_rows(it, row_list, sub, have);
+      }
       const uint32_t rows = it.rows, place0 = it.slot * p.tok;
       const uint32_t feature = my_tile(it) * kMxTileRows + 32 * sub + lane;
       const bool real = feature < p.w.rows;
@@ -778,7 +934,8 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
       // lane i of 16 knows the row of y of column c0 + i; fetched 16 columns ahead
       auto row_at = [&](uint32_t c) -> uint32_t {
         if (!p.experts) return place0 + c + (lane & 15u);
-        return c + (lane & 15u) < rows ? p.row_of[place0 + c + (lane & 15u)] : 0u;
+        if (c + (lane & 15u) >= rows) return 0u;
+        return FUSED ? row_list[c + (lane & 15u)] : p.row_of[place0 + c + (lane & 15u)];
       };
       uint32_t row_next = row_at(0);
       const uint32_t acc = item & 1u, d = tmem + (acc ? kMxAcc1 : 0u) + ((32u * sub) << 16);
@@ -872,7 +1029,7 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
 
 // --------------------------------------------------------------------- host
 struct MxPlan {
-  uint32_t tok, chunks, row_tiles, steps, split, in_block, pair, grid, stages, stage_bytes, x_step_bytes;
+  uint32_t tok, chunks, row_tiles, steps, split, in_block, pair, fused, x_resident, grid, stages, stage_bytes, x_step_bytes;
   uint64_t slots;
   uint64_t counters, slot_expert, slot_rows, row_of, place_of, x_packed, partial, bytes;
 };
@@ -881,9 +1038,12 @@ struct MxPlan {
 // product takes: an SM takes in some 50 bytes a cycle beside its products, all of them together 3400
 // from memory, the tensor cores need 2 cycles a row and step; what an item costs beside its steps and
 // what joining pieces costs grow with its rows.
-// `kind`: whole tiles, shared tiles, or tiles of a pair of CTAs, of which `sms` then counts the pairs.
-enum MxKind { kMxWhole, kMxShared, kMxPaired };
-static double mx_cost(uint64_t tok, double slots, const MxShape &w, double hit, uint32_t sms, MxKind kind) {
+// `kind`: whole tiles, shared tiles, tiles of a pair of CTAs, of which `sms` then counts the pairs, or whole
+// tiles whose CTAs quantise their rows themselves (for each slot they take, before its products) instead of a
+// kernel of its own.
+enum MxKind { kMxWhole, kMxShared, kMxPaired, kMxOneLaunch };
+static double mx_cost(uint64_t tok, double slots, const MxShape &w, double n_rows, double hit, uint32_t sms,
+                      MxKind kind) {
   const double pair = kind == kMxPaired ? 2 : 1;
   const double tiles = slots * ceil((double)w.row_tiles() / pair), steps = (double)w.steps();
   const double load = (kMxStepBytes + tok * 128.0 / pair + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 50.0;
@@ -895,10 +1055,18 @@ static double mx_cost(uint64_t tok, double slots, const MxShape &w, double hit, 
   };
   if (kind == kMxShared) {
     const double shares = 2 * tiles <= sms ? tiles * fmin(floor(sms / tiles), steps) : sms;
-    return ceil(tiles * steps / shares) * step(shares) + 3000 + 50.0 * tok;
+    return 5000 + ceil(tiles * steps / shares) * step(shares) + 3000 + 50.0 * tok;
   }
   const double waves = floor(tiles / sms), rest = tiles - waves * sms;
-  return waves * (steps * step(sms) + 300) + (rest > 0 ? steps * step(rest) + 300 : 0) + 8.0 * tok;
+  if (kind == kMxOneLaunch) {
+    const double rows = tok < n_rows / slots ? tok : n_rows / slots;
+    const double at_once = rows > 4 ? 8 : rows > 2 ? 4 : rows > 1 ? 2 : 1;
+    const double pieces = ceil(rows / at_once) * ceil((double)w.blocks() * at_once / 32);
+    const double quantise = 800 + ceil(pieces / (4 + kMxHelpers)) * 1200;
+    return ceil(tiles / sms) * quantise + waves * (steps * step(sms) + 300) + (rest > 0 ? steps * step(rest) + 300 : 0) +
+           8.0 * tok;
+  }
+  return 5000 + waves * (steps * step(sms) + 300) + (rest > 0 ? steps * step(rest) + 300 : 0) + 8.0 * tok;
 }
 
 // Pairs of CTAs that the device runs at a time.
@@ -914,21 +1082,27 @@ static bool mx_make_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan
   const double hit = grouped ? (double)w.matrices * (1 - pow(1 - 1.0 / (double)w.matrices, (double)n_rows)) : 1;
   uint64_t tok = 16;
   double best = -1;
-  g.split = g.pair = 0;
+  g.split = g.pair = g.fused = 0;
   for (uint64_t t = 16; t <= kMxMaxTok; t += 16) {
     double slots = grouped ? (double)n_rows / t + hit / 2 : ceil((double)n_rows / t);
     if (slots < hit) slots = hit;
-    for (MxKind kind : {kMxWhole, kMxShared, kMxPaired}) {
+    for (MxKind kind : {kMxWhole, kMxShared, kMxPaired, kMxOneLaunch}) {
       // steps times CTAs in 32 bits, and no more than a few tiles a CTA, or nothing is gained
       if (kind == kMxShared && (g.steps == 1 || slots * (double)w.row_tiles() * g.steps > 4e6)) continue;
       // the places of a pair's inputs depend on the slots' rows, which tables tell
       if (kind == kMxPaired && (g.in_block || n_pairs == 0)) continue;
-      const double cost = mx_cost(t, slots, w, hit, kind == kMxPaired ? n_pairs : sms, kind);
+      // a slot's rows beside four stages of W
+      if (kind == kMxOneLaunch && ((grouped && !g.in_block) ||
+                                   g.steps * (t * 128 + (t > 128 ? 2 : 1) * 2ull * kMxChunk) + 4 * kMxStepBytes >
+                                       kMaxDynamicSmem - 128 - kMxMiscBytes))
+        continue;
+      const double cost = mx_cost(t, slots, w, (double)n_rows, hit, kind == kMxPaired ? n_pairs : sms, kind);
       if (best < 0 || cost < best) {
         best = cost;
         tok = t;
         g.split = kind == kMxShared;
         g.pair = kind == kMxPaired;
+        g.fused = kind == kMxOneLaunch;
       }
     }
     if (t >= n_rows) break;
@@ -947,9 +1121,14 @@ static bool mx_make_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan
     g.grid = 2 * (uint32_t)(pairs < n_pairs ? pairs : n_pairs);
   }
   g.x_step_bytes = g.tok * 128 + g.chunks * 2 * kMxChunk;
-  g.stage_bytes = kMxStepBytes + (g.pair ? g.tok * 64 + g.chunks * 2 * kMxChunk : g.x_step_bytes);
-  g.stages = (kMaxDynamicSmem - 128 - kMxMiscBytes) / g.stage_bytes;
+  g.x_resident = g.fused ? g.steps * g.x_step_bytes : 0;
+  g.stage_bytes = kMxStepBytes + (g.fused  ? 0
+                                  : g.pair ? g.tok * 64 + g.chunks * 2 * kMxChunk
+                                           : g.x_step_bytes);
+  g.stages = (kMaxDynamicSmem - 128 - kMxMiscBytes - g.x_resident) / g.stage_bytes;
   if (g.stages > kMxMaxStages) g.stages = kMxMaxStages;
+  g.bytes = 0;
+  if (g.fused) return true;                    // no workspace
   uint64_t at = 256;
   auto take = [&](uint64_t bytes) {
     const uint64_t here = at;
@@ -1029,16 +1208,18 @@ static cudaError_t mx_device(uint32_t *pairs) {
   if (!d.ready) {
     const int most = (int)kMaxDynamicSmem;
     const auto larger = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    if ((err = cudaFuncSetAttribute(mx4_product_kernel<__nv_bfloat16, false>, larger, most)) != cudaSuccess ||
-        (err = cudaFuncSetAttribute(mx4_product_kernel<__half, false>, larger, most)) != cudaSuccess ||
-        (err = cudaFuncSetAttribute(mx4_product_kernel<__nv_bfloat16, true>, larger, most)) != cudaSuccess ||
-        (err = cudaFuncSetAttribute(mx4_product_kernel<__half, true>, larger, most)) != cudaSuccess ||
+    if ((err = cudaFuncSetAttribute(mx4_product_kernel<__nv_bfloat16, kMxFused>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_product_kernel<__half, kMxFused>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_product_kernel<__nv_bfloat16, kMxAlone>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_product_kernel<__half, kMxAlone>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_product_kernel<__nv_bfloat16, kMxPair>, larger, most)) != cudaSuccess ||
+        (err = cudaFuncSetAttribute(mx4_product_kernel<__half, kMxPair>, larger, most)) != cudaSuccess ||
         (err = cudaFuncSetAttribute(mx4_route_kernel, larger, (int)(kMxMaxExperts * 8))) != cudaSuccess)
       return err;
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = mx_config(2 * 1024, kMaxDynamicSmem, true, 0, attr);
     int clusters = 0;
-    if ((err = cudaOccupancyMaxActiveClusters(&clusters, mx4_product_kernel<__nv_bfloat16, true>, &cfg)) !=
+    if ((err = cudaOccupancyMaxActiveClusters(&clusters, mx4_product_kernel<__nv_bfloat16, kMxPair>, &cfg)) !=
         cudaSuccess)
       return err;
     d.pairs = (uint32_t)clusters;
@@ -1081,6 +1262,15 @@ template <typename T>
 static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
   MxPairMaps maps;
   memset(&maps, 0, sizeof(maps));
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = mx_config(
+      g.grid, 128 + g.x_resident + (size_t)p.stages * p.stage_bytes + kMxMiscBytes, p.pair != 0, st, attr);
+  if (g.fused) {
+    cfg.numAttrs = 0;
+    cfg.blockDim = dim3(mx_threads(kMxFused));
+    NZ_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, kMxFused>, p, maps));
+    return NZ_OK;
+  }
   if (p.pair) {
     const uint64_t x_rows = (uint64_t)p.slots * p.steps * p.x_step_bytes / 256;
     if (!mx_map(&maps.w, p.packed, p.w.bytes() / 256, kMxStepBytes / 256) ||
@@ -1092,26 +1282,23 @@ static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
   }
   uint32_t pairs = 0;
   NZ_CUDA_TRY(mx_device(&pairs));
-  const int wide = mx_wide_rows(p.x, p.x_stride, p.w.cols);
-  const uint64_t warps = (uint64_t)((p.n_rows / p.per_input + 7) / 8) * 2 * p.steps, blocks = (warps + 7) / 8;
+  const uint64_t rows = p.in_block ? p.n_rows : p.n_rows / p.per_input;
+  const uint64_t warps = (rows + 7) / 8 * 2 * p.steps, blocks = (warps + 7) / 8;
   const unsigned most = (unsigned)sm_count() * 8;
   const unsigned grid = blocks < most ? (unsigned)blocks : most;
-  auto rows_kernel = wide == 2   ? mx4_quantize_rows_kernel<T, 2>
-                     : wide == 1 ? mx4_quantize_rows_kernel<T, 1>
+  auto rows_kernel = p.wide == 2   ? mx4_quantize_rows_kernel<T, 2>
+                     : p.wide == 1 ? mx4_quantize_rows_kernel<T, 1>
                                  : mx4_quantize_rows_kernel<T, 0>;
   if (p.experts && !p.in_block) {
     mx4_route_kernel<<<1, kMxRouteThreads, p.w.matrices * 8, st>>>(p);
     NZ_LAUNCH_CHECK("mx4_route_kernel");
     NZ_CUDA_TRY(launch_dependent(rows_kernel, grid, 256, 0, st, p));
   } else {
-    rows_kernel<<<grid, 256, 0, st>>>(p);
+    rows_kernel<<<grid, 256, p.in_block ? sizeof(MxPlaces) : 0, st>>>(p);
     NZ_LAUNCH_CHECK("mx4_quantize_rows_kernel");
   }
-  cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg =
-      mx_config(g.grid, 128 + (size_t)p.stages * p.stage_bytes + kMxMiscBytes, p.pair != 0, st, attr);
-  NZ_CUDA_TRY(p.pair ? cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, true>, p, maps)
-                     : cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, false>, p, maps));
+  NZ_CUDA_TRY(p.pair ? cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, kMxPair>, p, maps)
+                     : cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, kMxAlone>, p, maps));
   return NZ_OK;
 }
 
@@ -1172,7 +1359,7 @@ extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t row
     set_error("nz_mx4_linear: the product of %llu rows is too large for one call", (unsigned long long)n_rows);
     return NZ_E_ARG;
   }
-  if (!workspace || workspace_bytes < g.bytes) {
+  if (workspace_bytes < g.bytes || (g.bytes && !workspace)) {
     set_error("nz_mx4_linear: workspace of %llu bytes is smaller than the %llu required",
               (unsigned long long)workspace_bytes, (unsigned long long)g.bytes);
     return NZ_E_CAPACITY;
@@ -1201,6 +1388,8 @@ extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t row
   p.split = g.split;
   p.in_block = g.in_block;
   p.pair = g.pair;
+  p.x_resident = g.x_resident;
+  p.wide = mx_wide_rows(x, x_stride, cols);
   p.stages = g.stages;
   p.stage_bytes = g.stage_bytes;
   p.wide_y = rows % 8 == 0 && ((uintptr_t)y & 15) == 0;

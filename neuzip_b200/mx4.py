@@ -33,11 +33,18 @@ class _Entry:
     rows: int
     cols: int
     packed: torch.Tensor      # uint8: codes and scales in the tensor cores' order
-    streams: set = field(default_factory=set)    # streams whose use the allocator knows of
+    streams: set              # streams whose use the allocator knows of
+    device: torch.device = field(init=False)
+
+    def __post_init__(self) -> None:
+        self.device = self.packed.device
 
     @property
     def numel(self) -> int:
         return self.matrices * self.rows * self.cols
+
+
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
 def _stack(shape: Sequence[int]):
@@ -100,10 +107,9 @@ class MX4Backend:
     def _use(self, entry: _Entry) -> int:
         """The current stream of the current device, which must be the entry's; from now on
         the allocator does not hand the entry's memory out while that stream may read it."""
-        device = entry.packed.get_device()
-        stream = torch._C._cuda_getCurrentRawStream(device)
+        stream = torch._C._cuda_getCurrentRawStream(entry.device.index)
         if stream not in entry.streams:
-            current = torch.cuda.current_stream(device)
+            current = torch.cuda.current_stream(entry.device)
             entry.packed.record_stream(current)
             entry.streams.add(stream)
         return stream
@@ -134,8 +140,8 @@ class MX4Backend:
 
     def read_shaped(self, name: str, shape) -> torch.Tensor:
         entry = self._get(name)
-        with torch.cuda.device(entry.packed.device):
-            out = torch.empty(entry.numel, dtype=entry.dtype, device=entry.packed.device).view(tuple(shape))
+        with torch.cuda.device(entry.device):
+            out = torch.empty(entry.numel, dtype=entry.dtype, device=entry.device).view(tuple(shape))
             _lib.check(self._lib.nz_mx4_dequantize(
                 _ptr(entry.packed), entry.matrices, entry.rows, entry.cols,
                 _DTYPES[entry.dtype], _ptr(out), self._use(entry)))
@@ -153,7 +159,7 @@ class MX4Backend:
             raise ValueError(f"row length {row_len} does not divide the {entry.numel} stored elements")
         if rows.is_floating_point() or rows.is_complex() or rows.dtype == torch.bool:
             raise TypeError(f"row numbers must be integers, got {rows.dtype}")
-        device = entry.packed.device
+        device = entry.device
         rows = rows.reshape(-1).to(device=device, dtype=torch.int64).contiguous()
         if row_len != entry.cols:
             # rows of several dimensions: each is a run of the table's own rows
@@ -175,21 +181,18 @@ class MX4Backend:
         return 0 if entry is None else entry.packed.numel()
 
     def linear(self, name: str, input: torch.Tensor, shape: Sequence[int],
-               bias: Optional[torch.Tensor]) -> torch.Tensor:
+               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``q(input) @ q(W)^T (+ bias)``: the inputs are quantised like the weights, sums are
         fp32, the result is rounded once to the type of `input`."""
         entry = self._get(name)
-        if len(shape) != 2 or entry.matrices != 1 or int(shape[0]) * int(shape[1]) != entry.numel \
-                or int(shape[1]) != entry.cols:
+        if len(shape) != 2 or entry.matrices != 1 or shape[1] != entry.cols or shape[0] != entry.rows:
             raise ValueError(f"linear needs a matrix, got a tensor of shape {tuple(shape)}")
         x = self._checked_input(entry, input, bias)
-        n_rows = x.shape[0]
         y = input.new_empty((*input.shape[:-1], entry.rows))
-        self._launch(entry, x, n_rows, 1, None, bias, y)
-        return y
+        return self._launch(entry, x, x.shape[0], 1, None, bias, y)
 
     def linear_without_bias(self, name: str, input: torch.Tensor, shape: Sequence[int]) -> torch.Tensor:
-        return self.linear(name, input, shape, None)
+        return self.linear(name, input, shape)
 
     def grouped_linear(self, name: str, input: torch.Tensor, experts: torch.Tensor,
                        bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -205,8 +208,8 @@ class MX4Backend:
                              f"got a tensor of shape {tuple(entry.shape)}")
         if experts.is_floating_point() or experts.is_complex() or experts.dtype == torch.bool:
             raise TypeError(f"expert numbers must be integers, got {experts.dtype}")
-        if experts.device != entry.packed.device:
-            raise ValueError(f"expert numbers are on {experts.device}, the weights on {entry.packed.device}")
+        if experts.device != entry.device:
+            raise ValueError(f"expert numbers are on {experts.device}, the weights on {entry.device}")
         lead, per_input = input.shape[:-1], 1
         if lead != experts.shape:
             if experts.dim() == 0 or lead != experts.shape[:-1]:
@@ -216,50 +219,54 @@ class MX4Backend:
         x = self._checked_input(entry, input, bias)
         ids = (experts if experts.dtype == torch.int64 else experts.long()).contiguous()
         y = input.new_empty((*experts.shape, entry.rows))
-        self._launch(entry, x, ids.numel(), per_input, ids, bias, y)
-        return y
+        return self._launch(entry, x, ids.numel(), per_input, ids, bias, y)
 
     def _checked_input(self, entry: _Entry, input: torch.Tensor,
                        bias: Optional[torch.Tensor]) -> torch.Tensor:
         """`input` as rows one element apart inside, after the checks the products share."""
         if input.dtype not in _DTYPES:
             raise RuntimeError("Unsupported data type")
-        if input.dim() < 1 or input.shape[-1] != entry.cols or entry.cols == 0:
-            raise ValueError(f"inputs of shape {tuple(input.shape)} do not fit weights of shape "
+        shape = input.shape
+        if not shape or shape[-1] != entry.cols or entry.cols == 0:
+            raise ValueError(f"inputs of shape {tuple(shape)} do not fit weights of shape "
                              f"{tuple(entry.shape)}")
-        if input.device != entry.packed.device:
-            raise ValueError(f"inputs are on {input.device}, the weights on {entry.packed.device}")
-        if bias is not None and (bias.dtype != input.dtype or bias.device != input.device
+        if input.device != entry.device:
+            raise ValueError(f"inputs are on {input.device}, the weights on {entry.device}")
+        if bias is not None and (bias.dtype != input.dtype or bias.device != entry.device
                                  or bias.numel() != entry.matrices * entry.rows):
             raise ValueError(f"bias must be {entry.matrices * entry.rows} numbers of type "
                              f"{_NAMES[input.dtype]} on {input.device}")
         if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
             raise RuntimeError("products with 4-bit weights have no gradient here: use nn.Linear, or "
                                "call under torch.no_grad()")
-        x = input.reshape(-1, entry.cols) if input.dim() != 2 else input
-        if x.stride(1) != 1 or x.stride(0) < entry.cols:
+        x = input if len(shape) == 2 else input.reshape(-1, entry.cols)
+        row, element = x.stride()
+        if element != 1 or row < entry.cols:
             x = x.contiguous()
         return x
 
     def _launch(self, entry: _Entry, x: torch.Tensor, n_rows: int, per_input: int,
-                ids: Optional[torch.Tensor], bias: Optional[torch.Tensor], y: torch.Tensor) -> None:
-        if y.numel() == 0:
-            return
-        device = x.get_device()
-        if device != torch.cuda.current_device():
+                ids: Optional[torch.Tensor], bias: Optional[torch.Tensor], y: torch.Tensor) -> torch.Tensor:
+        if n_rows == 0 or entry.rows == 0:
+            return y
+        device = entry.device.index
+        if device != _current_device():
             with torch.cuda.device(device):
                 return self._launch(entry, x, n_rows, per_input, ids, bias, y)
-        if bias is not None:
-            bias = bias.contiguous()
         need = _workspace_bytes(device, entry.matrices, entry.rows, entry.cols, n_rows, ids is not None)
         # from the allocator on every call: calls on other streams and captured graphs have their own
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        workspace = x.new_empty(need, dtype=torch.uint8) if need else None
+        if bias is not None:
+            bias = bias.contiguous()
+        status = self._status[device]
         rc = self._lib.nz_mx4_linear(
             entry.packed.data_ptr(), entry.matrices, entry.rows, entry.cols, _DTYPES[x.dtype], x.data_ptr(),
-            x.stride(0), n_rows, per_input, _ptr(ids), _ptr(bias), y.data_ptr(), _ptr(workspace), need,
-            self._status_of(device).data_ptr(), self._use(entry))
+            x.stride(0), n_rows, per_input, None if ids is None else ids.data_ptr(),
+            None if bias is None else bias.data_ptr(), y.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), need, status.data_ptr(), self._use(entry))
         if rc:
             _lib.check(rc)
+        return y
 
     def split(self, tensor: torch.Tensor):
         raise NotImplementedError("4-bit storage has no split()")

@@ -14,7 +14,7 @@ def manager_with(shape, name="w"):
     stack = _stack(shape)
     L = _lib.load()
     m._be._cache[name] = _Entry(torch.Size(shape), torch.bfloat16, *stack,
-                                torch.zeros(int(L.nz_mx4_bytes(*stack)), dtype=torch.uint8))
+                                torch.zeros(int(L.nz_mx4_bytes(*stack)), dtype=torch.uint8), set())
     m.meta_dict[name] = torch.Size(shape)
     return m
 
@@ -156,8 +156,9 @@ def test_library_refuses_bad_arguments():
     assert L.nz_mx4_gather_rows(16, 1, 1, 1, 0, 0, 1, 16, 0, 0) == _lib.NZ_E_ARG
     # product: stored bytes, matrices, rows, cols, dtype, x, stride, n_rows, per_input, experts, bias,
     # y, workspace, bytes, status, stream
-    good = [16, 1, 8, 64, 0, 16, 64, 40, 1, 0, 0, 16, 256, 1 << 30, 16, 0]
-    for at, value in ((0, 0), (0, 8), (2, 1 << 31), (4, 3), (5, 0), (5, 1), (6, 63), (8, 0), (8, 3), (1, 2),
+    good = [16, 1, 4096, 4096, 0, 16, 4096, 40000, 1, 0, 0, 16, 256, 1 << 32, 16, 0]
+    assert L.nz_mx4_linear_workspace_bytes(1, 4096, 4096, 40000, 0) > 0
+    for at, value in ((0, 0), (0, 8), (2, 1 << 31), (4, 3), (5, 0), (5, 1), (6, 4095), (8, 0), (8, 7), (1, 2),
                       (11, 0), (12, 16), (7, 1 << 31), (10, 1), (9, 4)):
         bad = list(good)
         bad[at] = value
