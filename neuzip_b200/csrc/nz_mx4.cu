@@ -12,6 +12,7 @@ constexpr int kMxThreads = 256;
 template <typename T, int WIDE>
 __global__ void __launch_bounds__(kMxThreads)
 mx4_quantize_kernel(const T *__restrict__ in, MxShape s, uint8_t *__restrict__ packed) {
+  __shared__ __align__(16) MxTurn turn[WIDE ? 1 : kMxThreads / 32];
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
   const uint32_t halves = 2 * (uint32_t)s.steps(), blocks = (uint32_t)s.blocks();
@@ -23,8 +24,14 @@ mx4_quantize_kernel(const T *__restrict__ in, MxShape s, uint8_t *__restrict__ p
     const uint64_t matrix = group / tile_groups;
     const uint32_t row = (uint32_t)(group - matrix * tile_groups) * 8 + (lane & 7u);
     uint32_t v[16], code[4], byte;
-    const int64_t left = row < s.rows ? (int64_t)s.cols - (int64_t)block * kMxBlock : 0;
-    mx_load_block<WIDE>(in + (matrix * s.rows + row) * s.cols + (uint64_t)block * kMxBlock, left, v);
+    const T *src = in + (matrix * s.rows + row) * s.cols;
+    if (WIDE) {
+      const int64_t left = row < s.rows ? (int64_t)s.cols - (int64_t)block * kMxBlock : 0;
+      mx_load_block<WIDE>(src + (uint64_t)block * kMxBlock, left, v);
+    } else {
+      const uint64_t first = (uint64_t)half * 128, left = s.cols > first ? s.cols - first : 0;
+      mx_load_turned(src + first, row < s.rows ? (uint32_t)(left < 128 ? left : 128) : 0, turn[threadIdx.x >> 5], v);
+    }
     mx_quantize_block<T>(v, code, byte);
     uint8_t *step = packed + (matrix * s.row_tiles() + row / kMxTileRows) * tile_bytes +
                     (uint64_t)(half >> 1) * kMxStepBytes;
@@ -74,26 +81,24 @@ template <typename T, int WIDE>
 __global__ void __launch_bounds__(kMxThreads)
 mx4_dequantize_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64_t *__restrict__ list,
                       uint64_t out_rows, T *__restrict__ out, uint32_t *status) {
+  __shared__ __align__(16) MxTurn turns[WIDE ? 1 : kMxThreads / 32];
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
   const uint32_t blocks = (uint32_t)s.blocks(), quads = (blocks + 3) / 4;
   const uint64_t total = (out_rows + 7) / 8 * quads;
   for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
     const uint64_t group = w / quads, to = group * 8 + (lane & 7u);
-    const uint32_t block = (uint32_t)(w - group * quads) * 4 + (lane >> 3);
-    if (block >= blocks || to >= out_rows) continue;
+    const uint32_t quad = (uint32_t)(w - group * quads), block = quad * 4 + (lane >> 3);
     uint64_t row;
     uint4 code = make_uint4(0, 0, 0, 0);
     uint32_t byte = 0;
-    if (mx_listed(list, s, to, row, status)) {
+    if (block < blocks && to < out_rows && mx_listed(list, s, to, row, status)) {
       const MxPlace at = mx_place(packed, s, row, block);
       code = __ldg(reinterpret_cast<const uint4 *>(at.codes));
       byte = __ldg(at.scale);
     }
     const float scale = mx_scale(byte);
     const uint32_t c[4] = {code.x, code.y, code.z, code.w};
-    T *dst = out + to * s.cols + (uint64_t)block * kMxBlock;
-    const uint64_t left = s.cols - (uint64_t)block * kMxBlock;
     uint32_t v[16];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -106,6 +111,28 @@ mx4_dequantize_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64
         memcpy(&v[4 * k + i], e, 4);
       }
     }
+    if (WIDE == 0) {
+      MxTurn &turn = turns[threadIdx.x >> 5];
+      __syncwarp();
+      uint4 *own = reinterpret_cast<uint4 *>(&turn.e[lane & 7u][(lane >> 3) * 32]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) own[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      __syncwarp();
+      const uint64_t first = (uint64_t)quad * 128;
+      const uint32_t n = (uint32_t)(s.cols - first < 128 ? s.cols - first : 128);
+      for (uint32_t j = 0; j < 8; j += 4) {
+        uint16_t *dst[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+          dst[k] = group * 8 + j + k < out_rows
+                       ? reinterpret_cast<uint16_t *>(out + (group * 8 + j + k) * s.cols + first) : nullptr;
+        mx_store_runs<4>(dst, turn.e[j], 136, n);
+      }
+      continue;
+    }
+    if (block >= blocks || to >= out_rows) continue;
+    T *dst = out + to * s.cols + (uint64_t)block * kMxBlock;
+    const uint64_t left = s.cols - (uint64_t)block * kMxBlock;
     if (WIDE == 2) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -119,42 +146,6 @@ mx4_dequantize_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64
       for (int h = 0; h < 4; ++h)
         if (left > 8 * h)
           *reinterpret_cast<uint4 *>(dst + 8 * h) = make_uint4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-    }
-  }
-}
-
-// The same where rows of the output are not aligned: a warp takes a row of up to eight blocks and
-// a lane one element of each, so that every store is 64 bytes in a piece (a block per thread, two
-// bytes at a time: 75 instead of 8 us for 1001 x 4099).
-template <typename T>
-__global__ void __launch_bounds__(kMxThreads)
-mx4_dequantize_odd_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64_t *__restrict__ list,
-                          uint64_t out_rows, T *__restrict__ out, uint32_t *status) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
-  const uint32_t blocks = (uint32_t)s.blocks(), steps = (uint32_t)s.steps();
-  const uint64_t total = out_rows * steps;
-  for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
-    const uint64_t to = w / steps;
-    const uint32_t first = (uint32_t)(w - to * steps) * 8;
-    uint64_t row;
-    const bool there = mx_listed(list, s, to, row, status);
-    uint32_t code[8], byte[8];
-#pragma unroll
-    for (uint32_t b = 0; b < 8; ++b) {
-      code[b] = byte[b] = 0;
-      if (there && first + b < blocks) {
-        const MxPlace at = mx_place(packed, s, row, first + b);
-        code[b] = __ldg(at.codes + (lane >> 1));
-        byte[b] = __ldg(at.scale);
-      }
-    }
-#pragma unroll
-    for (uint32_t b = 0; b < 8; ++b) {
-      const uint64_t col = (uint64_t)(first + b) * kMxBlock + lane;
-      if (col >= s.cols) break;
-      const float2 f = mx_decode2(code[b]);
-      out[to * s.cols + col] = from_float<T>(((lane & 1u) ? f.y : f.x) * mx_scale(byte[b]));
     }
   }
 }
@@ -217,9 +208,9 @@ static int dequantize(const void *packed, const nz::MxShape &s, const void *list
                       void *out, void *status, cudaStream_t st) {
   using namespace nz;
   const int wide = mx_wide_rows(out, s.cols, s.cols);
-  const uint64_t warps = wide ? (out_rows + 7) / 8 * ((s.blocks() + 3) / 4) : out_rows * s.steps();
+  const uint64_t warps = (out_rows + 7) / 8 * ((s.blocks() + 3) / 4);
   auto kern = wide == 2 ? mx4_dequantize_kernel<T, 2> : wide == 1 ? mx4_dequantize_kernel<T, 1>
-                                                                  : mx4_dequantize_odd_kernel<T>;
+                                                                  : mx4_dequantize_kernel<T, 0>;
   kern<<<mx_grid(warps), kMxThreads, 0, st>>>((const uint8_t *)packed, s, (const int64_t *)list, out_rows,
                                               (T *)out, (uint32_t *)status);
   NZ_LAUNCH_CHECK("mx4_dequantize_kernel");

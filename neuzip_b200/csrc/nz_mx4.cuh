@@ -125,6 +125,65 @@ __host__ __device__ __forceinline__ uint32_t mx_scale_offset(uint32_t r, uint32_
   return ((b >> 2) * chunks + (r >> 7)) * kMxChunk + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (b & 3u);
 }
 
+// Rows that are not even 16-byte aligned go through shared memory, eight rows of 128 columns a warp:
+// loads and stores of a warp are then runs of a row, and a thread still has a block.
+struct MxTurn {
+  uint16_t e[8][136];         // 272 bytes a row: the rows' blocks fall on different banks
+};
+// Lane l's block (l / 8) of row l % 8.  `src` is column 0 of the lane's row, `cols` how many there are.
+__device__ __forceinline__ void mx_load_turned(const void *src, uint32_t cols, MxTurn &t, uint32_t (&w)[16]) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint16_t v[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint16_t *row = (const uint16_t *)__shfl_sync(0xFFFFFFFFu, (unsigned long long)src, j);
+    const uint32_t n = __shfl_sync(0xFFFFFFFFu, cols, j);
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) v[j][c] = 32 * c + lane < n ? __ldg(row + 32 * c + lane) : 0;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) t.e[j][32 * c + lane] = v[j][c];
+  __syncwarp();
+  const uint4 *from = reinterpret_cast<const uint4 *>(&t.e[lane & 7u][(lane >> 3) * 32]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 q = from[i];
+    w[4 * i] = q.x;
+    w[4 * i + 1] = q.y;
+    w[4 * i + 2] = q.z;
+    w[4 * i + 3] = q.w;
+  }
+}
+// Runs of n <= 128 16-bit elements in shared memory to global memory, ROWS of them by a warp: two elements
+// a store, and one where a run begins or ends in the middle of a word.  All are read before any is
+// written (one by one, each waits for the one before: 250 cycles a run).  dst[k] is null for no run.
+template <int ROWS>
+__device__ __forceinline__ void mx_store_runs(uint16_t *const (&dst)[ROWS], const uint16_t *e, uint32_t apart,
+                                              uint32_t n) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t word[ROWS][2], ends[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const uint16_t *from = e + k * apart;
+    const uint32_t odd = (uint32_t)((uintptr_t)dst[k] >> 1) & 1u, at = 2 * lane + odd;
+    word[k][0] = (uint32_t)from[at] | (uint32_t)from[at + 1] << 16;
+    word[k][1] = (uint32_t)from[at + 64] | (uint32_t)from[at + 65 < 128 ? at + 65 : 127] << 16;
+    ends[k] = (uint32_t)from[0] | (uint32_t)from[n ? n - 1 : 0] << 16;
+  }
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    if (!dst[k]) continue;
+    const uint32_t odd = (uint32_t)((uintptr_t)dst[k] >> 1) & 1u, at = 2 * lane + odd;
+    if (at + 1 < n) *reinterpret_cast<uint32_t *>(dst[k] + at) = word[k][0];
+    if (at + 65 < n) *reinterpret_cast<uint32_t *>(dst[k] + at + 64) = word[k][1];
+    if (lane == 0 && odd && n) dst[k][0] = (uint16_t)ends[k];
+    if (lane == 31 && n > odd && ((n - odd) & 1u)) dst[k][n - 1] = (uint16_t)(ends[k] >> 16);
+  }
+}
+
 // The 32 elements of a block, of which `left` exist (the others are 0), as 16 words of two.
 // WIDE: 2 = the row is 32-byte aligned, 1 = 16-byte aligned, 0 = neither; left is a multiple of
 // 16, of 8, anything.

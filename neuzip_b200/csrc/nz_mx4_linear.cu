@@ -58,7 +58,7 @@ struct MxLinearArgs {
   uint32_t *counters;         // split: arrivals at every tile
   uint32_t *slot_expert, *slot_rows;       // stack: matrix of a slot, rows in it
   uint32_t *row_of;           // stack: row of y at every place of the slots
-  uint32_t *place_of;         // stack: place of every row of y, kMxNone without a matrix
+  uint2 *place_of;            // stack: see MxWhere, of every row of y
   uint8_t *x_packed;
   float *partial;             // split: two pieces [tok][128] of every CTA
 };
@@ -247,6 +247,26 @@ __device__ __forceinline__ bool mx_store_all(bool ok) {
   return r != 0;
 }
 
+// Columns of a product for so many rows of x.
+__device__ __forceinline__ uint32_t mx_columns(uint32_t rows) { return (rows + 15u) & ~15u; }
+
+// Where a row of x goes: its slot (kMxNone: nowhere); in its low half the row's number in the slot, in its
+// high half its place among the codes of a step's first block.  For a pair of CTAs the first half of
+// the product's columns lies by itself before the second one.
+struct MxWhere {
+  uint32_t slot, at;
+  __device__ __forceinline__ uint32_t row() const { return at & 0xFFFFu; }
+  __device__ __forceinline__ uint32_t code() const { return at >> 16; }
+};
+__device__ __forceinline__ uint2 mx_where(const MxLinearArgs &p, uint32_t slot, uint32_t i, uint32_t rows) {
+  uint32_t code = i;
+  if (p.pair) {
+    const uint32_t split = mx_columns(rows) / 2;
+    if (i >= split) code = 8 * (p.tok / 2) + i - split;
+  }
+  return make_uint2(slot, code << 16 | i);
+}
+
 // ------------------------------------------------------------------ rows in order of their matrix
 // One block.  Counts the rows of every matrix, gives each matrix as many slots as it fills, then
 // gives every row a place.  Which rows of a matrix come first is open; no result depends on it.
@@ -293,6 +313,7 @@ __global__ void __launch_bounds__(kMxRouteThreads) mx4_route_kernel(const MxLine
     const uint32_t first = before + sum - mine;
     if (e < experts) {
       next[e] = first * p.tok;
+      count[e] = rows + first * p.tok;             // one past its last place, were its slots without gaps
       for (uint32_t k = 0; k < mine; ++k) {
         p.slot_expert[first + k] = e;
         p.slot_rows[first + k] = rows - k * p.tok < p.tok ? rows - k * p.tok : p.tok;
@@ -312,12 +333,13 @@ __global__ void __launch_bounds__(kMxRouteThreads) mx4_route_kernel(const MxLine
     for (int i = 0; i < kMxRouteBatch; ++i) {
       const uint64_t r = r0 + i * kMxRouteThreads;
       if (r >= p.n_rows) continue;
-      uint32_t place = kMxNone;
+      uint2 where = make_uint2(kMxNone, 0);
       if (e[i] >= 0 && e[i] < (int64_t)experts) {
-        place = atomicAdd(&next[e[i]], 1u);
+        const uint32_t place = atomicAdd(&next[e[i]], 1u), slot = place / p.tok;
         p.row_of[place] = (uint32_t)r;
+        where = mx_where(p, slot, place - slot * p.tok, min(p.tok, count[e[i]] - slot * p.tok));
       }
-      p.place_of[r] = place;
+      p.place_of[r] = where;
     }
   }
 }
@@ -446,9 +468,6 @@ __device__ __forceinline__ void mx_list_rows(const MxLinearArgs &p, const uint16
   __syncwarp();
 }
 
-// Columns of a product for so many rows of x.
-__device__ __forceinline__ uint32_t mx_columns(uint32_t rows) { return (rows + 15u) & ~15u; }
-
 // ------------------------------------------------------------------ the rows of x
 // As in mx4_quantize_kernel a thread takes a block, a warp eight rows of x of four blocks.  A row is
 // quantised once and written to the place of every row of y it serves.  Rows of y without a matrix
@@ -456,6 +475,7 @@ __device__ __forceinline__ uint32_t mx_columns(uint32_t rows) { return (rows + 1
 template <typename T, int WIDE>
 __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearArgs p) {
   extern __shared__ uint32_t rows_smem[];
+  __shared__ __align__(16) MxTurn turn[WIDE ? 1 : 8];
   MxPlaces &places = *reinterpret_cast<MxPlaces *>(rows_smem);       // in_block
   // The product is let in when everything before this kernel is complete, W among it: it begins to
   // read W while this kernel runs.
@@ -469,38 +489,61 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
   // Items are rows of x, or where there are few of them rows of y: then a row of x that serves several
   // is quantised for each, by warps of their own.
   const uint32_t serves = p.in_block ? 1 : p.per_input, shared = p.per_input / serves;
+  constexpr uint32_t kAhead = 4;
+  const uint32_t apart = p.pair ? p.tok / 2 : p.tok;            // rows of a block of codes
   const uint32_t halves = 2 * p.steps, inputs = p.n_rows / serves;
   const uint64_t total = (uint64_t)((inputs + 7) / 8) * halves;
   for (uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (uint64_t)gridDim.x * 8) {
     const uint32_t group = (uint32_t)(w / halves), half = (uint32_t)(w - (uint64_t)group * halves);
     const uint32_t row = group * 8 + (lane & 7u), block = half * 4 + (lane >> 3);
     uint32_t v[16], code[4], byte;
-    const int64_t left = row < inputs ? (int64_t)p.w.cols - (int64_t)block * kMxBlock : 0;
-    mx_load_block<WIDE>((const T *)p.x + row / shared * p.x_stride + (uint64_t)block * kMxBlock, left, v);
+    // where the row goes, known before the row is there
+    uint2 where[kAhead];
+    auto find = [&](uint32_t j0) {
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; ++j) {
+        const uint32_t r = row * serves + j0 + j;
+        if (row >= inputs || j0 + j >= serves) continue;
+        if (p.in_block || !p.experts) {
+          const uint32_t place = p.in_block ? places.place[r] : r, slot = place / p.tok;
+          where[j] = place == kMxNone ? make_uint2(kMxNone, 0)
+                                      : mx_where(p, slot, place - slot * p.tok, min(p.tok, p.n_rows - slot * p.tok));
+        } else {
+          where[j] = __ldcg(p.place_of + r);
+        }
+      }
+    };
+    find(0);
+    const T *src = (const T *)p.x + row / shared * p.x_stride;
+    if (WIDE) {
+      const int64_t left = row < inputs ? (int64_t)p.w.cols - (int64_t)block * kMxBlock : 0;
+      mx_load_block<WIDE>(src + (uint64_t)block * kMxBlock, left, v);
+    } else {
+      const uint64_t first = (uint64_t)half * 128, left = p.w.cols > first ? p.w.cols - first : 0;
+      mx_load_turned(src + first, row < inputs ? (uint32_t)(left < 128 ? left : 128) : 0, turn[threadIdx.x >> 5], v);
+    }
     mx_quantize_block<T>(v, code, byte);
     const uint32_t word = mx_pack_scales(byte, lane);
     if (row >= inputs) continue;
-    for (uint32_t j = 0; j < serves; ++j) {
-      const uint32_t r = row * serves + j;
-      const uint32_t place = p.in_block ? places.place[r] : p.experts ? p.place_of[r] : r;
-      if (place == kMxNone) {
+    for (uint32_t j0 = 0; j0 < serves; j0 += kAhead) {
+      if (j0) find(j0);
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; ++j) {
+      if (j0 + j >= serves) break;
+      const uint32_t r = row * serves + j0 + j;
+      const MxWhere to{where[j].x, where[j].y};
+      if (to.slot == kMxNone) {
         // the row's lanes of all its warps share it out
         const uint64_t n = p.w.rows;
         for (uint64_t i = block; i < n; i += 4 * halves) ((T *)p.y)[r * n + i] = from_float<T>(0.f);
         continue;
       }
-      const uint32_t slot = place / p.tok, i = place - slot * p.tok;
-      uint8_t *step = p.x_packed + ((uint64_t)slot * p.steps + (half >> 1)) * p.x_step_bytes;
-      uint32_t at = (block & 7u) * p.tok + i;
-      if (p.pair) {
-        // the first half of the product's columns, then the second, each on its own
-        const uint32_t rows = p.experts ? __ldcg(p.slot_rows + slot) : min(p.tok, p.n_rows - slot * p.tok);
-        const uint32_t split = mx_columns(rows) / 2, second = i >= split;
-        at = (8 * second + (block & 7u)) * (p.tok / 2) + i - second * split;
-      }
-      *reinterpret_cast<uint4 *>(step + at * 16) = make_uint4(code[0], code[1], code[2], code[3]);
+      uint8_t *step = p.x_packed + ((uint64_t)to.slot * p.steps + (half >> 1)) * p.x_step_bytes;
+      *reinterpret_cast<uint4 *>(step + ((block & 7u) * apart + to.code()) * 16) =
+          make_uint4(code[0], code[1], code[2], code[3]);
       if (lane < 8)
-        *reinterpret_cast<uint32_t *>(step + 128 * p.tok + mx_scale_offset(i, (half & 1) * 4, p.chunks)) = word;
+        *reinterpret_cast<uint32_t *>(step + 128 * p.tok + mx_scale_offset(to.row(), (half & 1) * 4, p.chunks)) = word;
+      }
     }
   }
 }
@@ -885,7 +928,7 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
     dependent_wait();
     MxItems items(p, table, slots_now());
     const uint32_t sub = warp & 3u;                   // tensor-memory lanes 32 sub .. + 31
-    T *turn = reinterpret_cast<T *>(misc + kMxTurn) + sub * 512;
+    T *const turns = reinterpret_cast<T *>(misc + kMxTurn), *const turn = turns + sub * 512;
     uint16_t *row_list = reinterpret_cast<uint16_t *>(misc + kMxRowList) + sub * 256;
     if (FUSED && p.in_block) {
       // rows of y without a matrix
@@ -924,11 +967,23 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
           }
           __syncwarp();
         } else {
+          // Rows begin anywhere.  The four warps put their 32 features together, then each stores four
+          // rows of all 128: a sector that is written in parts costs a read as well, and so a row has two
+          // of them instead of eight.
 #pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) {
+          for (uint32_t i = 0; i < 16; ++i) turns[i * 128 + 32 * sub + lane] = from_float<T>(f[i] + bias);
+          mx_store_barrier();
+          const uint32_t first = my_tile(it) * kMxTileRows;
+          const uint32_t n = first < p.w.rows ? min(kMxTileRows, (uint32_t)p.w.rows - first) : 0;
+          uint16_t *dst[4];
+#pragma unroll
+          for (uint32_t h = 0; h < 4; ++h) {
+            const uint32_t i = 4 * sub + h;
             const uint64_t r = __shfl_sync(0xFFFFFFFFu, row_here, i);
-            if (i < count && real) y[r * p.w.rows + lane] = from_float<T>(f[i] + bias);
+            dst[h] = i < count ? reinterpret_cast<uint16_t *>(y - 32 * sub + r * p.w.rows) : nullptr;
           }
+          mx_store_runs<4>(dst, reinterpret_cast<uint16_t *>(turns + 4 * sub * 128), 128, n);
+          mx_store_barrier();
         }
       };
       // lane i of 16 knows the row of y of column c0 + i; fetched 16 columns ahead
@@ -1140,7 +1195,7 @@ static bool mx_make_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan
   g.slot_expert = take(tables ? g.slots * 4 : 0);
   g.slot_rows = take(tables ? g.slots * 4 : 0);
   g.row_of = take(grouped ? g.slots * tok * 4 : 0);
-  g.place_of = take(tables ? n_rows * 4 : 0);
+  g.place_of = take(tables ? n_rows * 8 : 0);
   g.x_packed = take(g.slots * g.steps * g.x_step_bytes);
   g.partial = take(g.split ? (uint64_t)g.grid * 2 * tok * kMxTileRows * 4 : 0);
   g.bytes = at;
@@ -1398,7 +1453,7 @@ extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t row
   p.slot_expert = (uint32_t *)(ws + g.slot_expert);
   p.slot_rows = (uint32_t *)(ws + g.slot_rows);
   p.row_of = (uint32_t *)(ws + g.row_of);
-  p.place_of = (uint32_t *)(ws + g.place_of);
+  p.place_of = (uint2 *)(ws + g.place_of);
   p.x_packed = ws + g.x_packed;
   p.partial = (float *)(ws + g.partial);
   return dtype == NZ_DTYPE_BF16 ? mx_launch<__nv_bfloat16>(p, g, (cudaStream_t)stream)
