@@ -69,28 +69,30 @@ __device__ __forceinline__ float mx_inverse_scale(uint32_t byte) {
 __device__ __forceinline__ float mx_scale(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7FFFFFFFu : byte ? byte << 23 : 0x00400000u);
 }
-// Two magnitudes to codes, the first in the low half; the instruction saturates at 6 and rounds
-// ties to even.
-__device__ __forceinline__ uint32_t mx_encode2(float lo, float hi) {
+// Eight numbers to a word of codes, the first in the lowest bits; the instruction saturates at 6 and
+// rounds ties to even.
+__device__ __forceinline__ uint32_t mx_encode8(const float2 (&f)[4]) {
   uint32_t r;
-  asm("{\n\t.reg .b8 b;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\t"
-      "cvt.u32.u8 %0, b;\n\t}"
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
       : "=r"(r)
-      : "f"(lo), "f"(hi));
+      : "f"(f[0].x), "f"(f[0].y), "f"(f[1].x), "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x), "f"(f[3].y));
   return r;
 }
-// The two numbers of a byte, the low half first.
-__device__ __forceinline__ float2 mx_decode2(uint32_t byte) {
-  uint32_t h;
-  asm("{\n\t.reg .b8 b;\n\t"
-      "cvt.u8.u32 b, %1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
-      : "=r"(h)
-      : "r"(byte));
-  __half2 v;
-  memcpy(&v, &h, 4);
-  return __half22float2(v);
+// The eight numbers of a word of codes as four pairs of fp16, which holds them exactly.
+__device__ __forceinline__ void mx_decode8(uint32_t word, uint32_t (&pair)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(pair[0]), "=r"(pair[1]), "=r"(pair[2]), "=r"(pair[3])
+      : "r"(word));
 }
 
 // Checks that the entry points share (they set the error text).
@@ -107,18 +109,6 @@ inline int mx_wide_rows(const void *p, uint64_t stride, uint64_t cols) {
 bool mx_few_rows(const MxShape &w, uint64_t n_rows, bool grouped);
 int mx_few(const MxShape &w, int dtype, const void *packed, const void *x, uint64_t x_stride, uint64_t n_rows,
            uint64_t per_input, const void *experts, const void *bias, void *y, void *status, cudaStream_t st);
-
-// The eight numbers of a word of codes as four pairs of fp16, which holds them exactly.
-__device__ __forceinline__ void mx_decode8(uint32_t word, uint32_t (&pair)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "mov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(pair[0]), "=r"(pair[1]), "=r"(pair[2]), "=r"(pair[3])
-      : "r"(word));
-}
 
 // Offset of the scale of row r (in a tile of up to 128 * chunks rows), block b of the step.
 __host__ __device__ __forceinline__ uint32_t mx_scale_offset(uint32_t r, uint32_t b, uint32_t chunks) {
@@ -228,26 +218,32 @@ __device__ __forceinline__ float2 mx_unpack2<__half>(uint32_t w) {
   memcpy(&h, &w, 4);
   return __half22float2(h);
 }
+// The fp32 bits of the largest of two 16-bit magnitudes (which are ordered like whole numbers).
+template <typename T> __device__ __forceinline__ uint32_t mx_largest_bits(uint32_t pair);
+template <> __device__ __forceinline__ uint32_t mx_largest_bits<__nv_bfloat16>(uint32_t pair) {
+  return max(pair & 0xFFFF0000u, pair << 16);
+}
+template <> __device__ __forceinline__ uint32_t mx_largest_bits<__half>(uint32_t pair) {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(pair >> 16, pair & 0xFFFFu)))) & 0x7FFFFFFFu;
+}
 // Codes and scale byte of a block.
 template <typename T>
 __device__ __forceinline__ void mx_quantize_block(const uint32_t (&w)[16], uint32_t (&code)[4], uint32_t &byte) {
   uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float2 f = mx_unpack2<T>(w[i]);
-    a = max(a, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
-  }
-  byte = mx_scale_byte(a);
+  for (int i = 0; i < 16; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(a) : "r"(w[i] & 0x7FFF7FFFu));
+  byte = mx_scale_byte(mx_largest_bits<T>(a));
   const float inv = mx_inverse_scale(byte);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t c = 0;
+    float2 f[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 f = mx_unpack2<T>(w[4 * i + j]);
-      c |= mx_encode2(f.x * inv, f.y * inv) << (8 * j);
+      f[j] = mx_unpack2<T>(w[4 * i + j]);
+      f[j].x *= inv;
+      f[j].y *= inv;
     }
-    code[i] = byte == 255u ? 0u : c;
+    code[i] = byte == 255u ? 0u : mx_encode8(f);
   }
 }
 // The scale bytes of the four blocks of 128 columns, which lanes l, l + 8, l + 16, l + 24 hold, as
