@@ -477,9 +477,8 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
   extern __shared__ uint32_t rows_smem[];
   __shared__ __align__(16) MxTurn turn[WIDE ? 1 : 8];
   MxPlaces &places = *reinterpret_cast<MxPlaces *>(rows_smem);       // in_block
-  // The product is let in when everything before this kernel is complete, W among it: it begins to
-  // read W while this kernel runs.
-  dependent_wait();
+  // The product may come in now.  All that was launched before this kernel is complete (its own launch is
+  // an ordinary one), W among it, which the product begins to read while this kernel runs.
   dependent_trigger();
   const uint32_t lane = threadIdx.x & 31;
   if (p.in_block) mx_find_places(p, places);
@@ -529,20 +528,21 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
       if (j0) find(j0);
 #pragma unroll
       for (uint32_t j = 0; j < kAhead; ++j) {
-      if (j0 + j >= serves) break;
-      const uint32_t r = row * serves + j0 + j;
-      const MxWhere to{where[j].x, where[j].y};
-      if (to.slot == kMxNone) {
-        // the row's lanes of all its warps share it out
-        const uint64_t n = p.w.rows;
-        for (uint64_t i = block; i < n; i += 4 * halves) ((T *)p.y)[r * n + i] = from_float<T>(0.f);
-        continue;
-      }
-      uint8_t *step = p.x_packed + ((uint64_t)to.slot * p.steps + (half >> 1)) * p.x_step_bytes;
-      *reinterpret_cast<uint4 *>(step + ((block & 7u) * apart + to.code()) * 16) =
-          make_uint4(code[0], code[1], code[2], code[3]);
-      if (lane < 8)
-        *reinterpret_cast<uint32_t *>(step + 128 * p.tok + mx_scale_offset(to.row(), (half & 1) * 4, p.chunks)) = word;
+        if (j0 + j >= serves) break;
+        const MxWhere to{where[j].x, where[j].y};
+        if (to.slot == kMxNone) {
+          // the row's lanes of all its warps share it out
+          const uint64_t n = p.w.rows;
+          T *y = (T *)p.y + (uint64_t)(row * serves + j0 + j) * n;
+          for (uint64_t i = block; i < n; i += 4 * halves) y[i] = from_float<T>(0.f);
+          continue;
+        }
+        uint8_t *step = p.x_packed + ((uint64_t)to.slot * p.steps + (half >> 1)) * p.x_step_bytes;
+        *reinterpret_cast<uint4 *>(step + ((block & 7u) * apart + to.code()) * 16) =
+            make_uint4(code[0], code[1], code[2], code[3]);
+        if (lane < 8)
+          *reinterpret_cast<uint32_t *>(step + 128 * p.tok + mx_scale_offset(to.row(), (half & 1) * 4, p.chunks)) =
+              word;
       }
     }
   }
@@ -1036,9 +1036,9 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
         // The CTA that brings the last piece of a tile adds all of them, in the order of the steps.
         const uint32_t first = items.owner(it.tile * p.steps);
         const uint32_t pieces = items.owner(it.tile * p.steps + p.steps - 1) - first + 1;
-        __threadfence();
         mx_store_barrier();
         if (threadIdx.x == 64) {
+          __threadfence();                            // cumulative: the warps' stores, then the arrival
           const uint32_t seen = atomicAdd(p.counters + it.tile, 1u);
           __threadfence();
           *last_flag = seen == pieces - 1;
@@ -1347,11 +1347,9 @@ static int mx_launch(const MxLinearArgs &p, const MxPlan &g, cudaStream_t st) {
   if (p.experts && !p.in_block) {
     mx4_route_kernel<<<1, kMxRouteThreads, p.w.matrices * 8, st>>>(p);
     NZ_LAUNCH_CHECK("mx4_route_kernel");
-    NZ_CUDA_TRY(launch_dependent(rows_kernel, grid, 256, 0, st, p));
-  } else {
-    rows_kernel<<<grid, 256, p.in_block ? sizeof(MxPlaces) : 0, st>>>(p);
-    NZ_LAUNCH_CHECK("mx4_quantize_rows_kernel");
   }
+  rows_kernel<<<grid, 256, p.in_block ? sizeof(MxPlaces) : 0, st>>>(p);
+  NZ_LAUNCH_CHECK("mx4_quantize_rows_kernel");
   NZ_CUDA_TRY(p.pair ? cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, kMxPair>, p, maps)
                      : cudaLaunchKernelEx(&cfg, mx4_product_kernel<T, kMxAlone>, p, maps));
   return NZ_OK;

@@ -77,6 +77,7 @@ class MX4Backend:
         self._lib = _lib.load()
         self._cache: Dict[str, _Entry] = {}
         self._status: Dict[int, torch.Tensor] = {}
+        self._captured: Dict[int, torch.Tensor] = {}     # bytes that a captured graph reads
 
     # -- helpers ---------------------------------------------------------
     def _status_of(self, device: int) -> torch.Tensor:
@@ -108,6 +109,9 @@ class MX4Backend:
         """The current stream of the current device, which must be the entry's; from now on
         the allocator does not hand the entry's memory out while that stream may read it."""
         stream = torch._C._cuda_getCurrentRawStream(entry.device.index)
+        if torch._C._cuda_isCurrentStreamCapturing():
+            # the graph reads these bytes at every replay, whatever becomes of the handle
+            self._captured[entry.packed.data_ptr()] = entry.packed
         if stream not in entry.streams:
             current = torch.cuda.current_stream(entry.device)
             entry.packed.record_stream(current)
