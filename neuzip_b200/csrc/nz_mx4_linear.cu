@@ -1,13 +1,38 @@
 // y = q(x) q(W)^T (+ bias) with both operands in microscaled 4-bit floating point, W one matrix or
 // a stack of which every row of the result names one (a mixture-of-experts layer).
 //
-// The tensor cores take the stored form as it is: tcgen05.mma kind::mxf4 multiplies 4-bit operands
-// from shared memory, scales from tensor memory, and adds in fp32.  Kernels of a call:
-//   route      (stack only) puts the rows of y in order of their matrix, in "slots" of p.tok rows
-//              of which all have the same matrix; the last slot of a matrix is not full
-//   quantise   turns the rows of x into codes and scales, in slot order, in the workspace
-//   product    one work item = (slot, tile of 128 rows of W, range of steps of 256 columns)
-// A tile of W is the M side of the MMA (128 tensor-memory lanes), a slot the N side (its columns).
+// The tensor cores take the stored form as it is: tcgen05.mma kind::mxf4 multiplies 4-bit operands from
+// shared memory with their scales from tensor memory and adds in fp32 there.  Rows of x that share a
+// matrix are brought together in "slots" of up to p.tok (a dense product has slots too).  A tile of
+// 128 rows of W is the M side of the products (tensor-memory lanes), a slot the N side (columns), a step
+// 256 columns of both.  A step of a tile of W lies in one piece (nz_mx4.cuh): a bulk copy fetches it, no
+// tensor map is needed, and memory is read in runs of 17 KB.
+//
+// One persistent CTA an SM: a thread that copies, a thread that issues, four warps that store.  Steps go
+// through a ring of stages (full[s]: bytes have arrived, empty[s]: tcgen05.commit); two accumulators
+// let the products of a tile run while the one before is stored.  Each of the two loops is one thread's,
+// taken by elect.sync: under `lane == 0` the compiler moves every operand of an instruction across
+// the warp first, and a step took 1000 cycles to issue instead of 300.
+//
+// Ways of running, chosen by an estimate of their times (mx_cost) from sizes alone:
+//   few     (nz_mx4_few.cu) one or two rows, or some rows of a stack, on the CUDA cores
+//   fused   one launch; every CTA quantises the rows of its slots itself, into shared memory, by 12 warps.
+//           The less host time (one launch, no workspace), and no longer up to about 4 rows of 4096
+//   alone   a kernel quantises x into the workspace, and the product reads W meanwhile (a programmatic
+//           dependent launch): its ring is full of W when the inputs come
+//   shared  the same, and the steps of all tiles are divided evenly over the SMs, not tiles; the CTA that
+//           finishes a tile last adds its pieces in the order of the steps, so that bits do not depend on
+//           who is last
+//   pair    two CTAs with cta_group::2: 256 rows of W, half of a slot's step each.  A step then brings 34
+//           instead of 51 KB into an SM.  Large products are bound by that traffic and the power it
+//           takes: 8192 x 8192 x 28672 took 1293 us alone and takes 790 in pairs under sustained load, and
+//           580 if nothing but scales were copied
+// Rows find their slots in every block (up to 1024 rows and 256 matrices) or by a kernel of one block.
+//
+// Measured on a B200, cold weights, in a graph (the bytes at 6.54 TB/s in brackets, in us): 16 rows x 4096
+// x 11008 9.5 (3.7), 8192 x 8192 13.2 (5.4), 8192 x 28672 26.0 (19.1); 64 experts 1408 x 2048, 32 tokens
+// to 8 each 23.3 (14.8).  What is over the bytes is a constant 6 to 7 us: two launches (2), the first
+// bytes' latency (2), the last step's products and stores (1), the end of the grid (1).
 #include <cuda.h>
 #include <math.h>
 #include <string.h>
@@ -46,7 +71,8 @@ struct MxLinearArgs {
   uint32_t slots;             // slots there can be
   uint32_t row_tiles, steps, blocks;
   uint32_t x_step_bytes;      // a step of a slot: codes, scales
-  uint32_t split;             // 1: the steps of a tile may be shared between CTAs
+  uint32_t split;             // > 0: the steps of a tile may be shared, where there are two CTAs or more for
+                              // every tile between this many
   uint32_t in_block;          // stack: few rows of y, which every block groups by itself
   uint32_t pair;              // 1: two CTAs share a slot's step and take two tiles of W
   uint32_t x_resident;        // bytes of a slot's steps in shared memory, quantised there; else 0
@@ -573,7 +599,7 @@ struct MxItems {
     if (p.split) {
       const uint32_t units = tiles * p.steps;
       shares = gridDim.x;
-      if (tiles && 2 * tiles <= gridDim.x) shares = tiles * min(gridDim.x / tiles, p.steps);
+      if (tiles && 2 * tiles <= gridDim.x) shares = tiles * min(min(gridDim.x / tiles, p.steps), p.split);
       if (shares > units) shares = units;
       at = end = 0;
       if (blockIdx.x < shares) {
@@ -1084,44 +1110,59 @@ mx4_product_kernel(const MxLinearArgs p, const __grid_constant__ MxPairMaps maps
 
 // --------------------------------------------------------------------- host
 struct MxPlan {
-  uint32_t tok, chunks, row_tiles, steps, split, in_block, pair, fused, x_resident, grid, stages, stage_bytes, x_step_bytes;
+  uint32_t tok, chunks, row_tiles, steps, split, in_block, pair, fused, pieces, x_resident, grid, stages, stage_bytes, x_step_bytes;
   uint64_t slots;
   uint64_t counters, slot_expert, slot_rows, row_of, place_of, x_packed, partial, bytes;
 };
 
-// The rows of a slot, and whether tiles are shared, by an estimate of the time (in cycles) that the
-// product takes: an SM takes in some 50 bytes a cycle beside its products, all of them together 3400
-// from memory, the tensor cores need 2 cycles a row and step; what an item costs beside its steps and
-// what joining pieces costs grow with its rows.
+// The rows of a slot and the way of running, by an estimate of the time (in cycles) that a call takes.
 // `kind`: whole tiles, shared tiles, tiles of a pair of CTAs, of which `sms` then counts the pairs, or whole
 // tiles whose CTAs quantise their rows themselves (for each slot they take, before its products) instead of a
 // kernel of its own.
+// A step takes the longest of: its products (2 cycles a row), their issuing (420), its bytes into an SM (80
+// a cycle) and into all of them (7400 from L2; 3400 of W from memory).  A launch before the product costs
+// 5000 (its device time is hidden in part, its host time is not), a pair's start 2000 more, an item beside
+// its steps 300 and 8 a row.  The pieces of a shared tile are joined four at a time, 16 columns in 1800.
+// Against measurements, in us, this way and the next best: 16 rows x 4096 x 11008 alone 9.5, fused 14.0;
+// 4 rows fused 10.0, alone 9.6 and 4 more of host time; 4 rows x 8192 x 512 shared by a few CTAs a tile 9.4,
+// by 32 18.2, in whole tiles 11.9; 256 rows x 16384 x 2048 whole 21.9, shared 32.5; 4 rows x 16384 x 2048 shared 17.0,
+// whole 27.9; 2048 rows x 8192 x 28672 in pairs 190, alone 280; 64 rows x 4096 x 11008 alone 10.1, in pairs 11.1.
 enum MxKind { kMxWhole, kMxShared, kMxPaired, kMxOneLaunch };
 static double mx_cost(uint64_t tok, double slots, const MxShape &w, double n_rows, double hit, uint32_t sms,
-                      MxKind kind) {
+                      MxKind kind, uint32_t &pieces) {
   const double pair = kind == kMxPaired ? 2 : 1;
   const double tiles = slots * ceil((double)w.row_tiles() / pair), steps = (double)w.steps();
-  const double load = (kMxStepBytes + tok * 128.0 / pair + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk) / 50.0;
-  const double mma = 2.0 * tok, busy = load > mma ? load : mma;
-  // a step's share of what comes from memory, with so many tiles at work: slots of a matrix share it
+  const double bytes = kMxStepBytes + tok * 128.0 / pair + (tok > 128 ? 2 : 1) * 2.0 * kMxChunk;
+  // with so many tiles at work; slots of a matrix share what comes from memory
   auto step = [&](double active) {
-    const double memory = pair * kMxStepBytes * (hit / slots) * active / 3400.0;
-    return busy > memory ? busy : memory;
+    double longest = fmax(fmax(2.0 * tok, 420), bytes / 80);
+    longest = fmax(longest, bytes * pair * active / 7400);
+    return fmax(longest, pair * kMxStepBytes * (hit / slots) * active / 3400);
   };
+  const double item = 300 + 8.0 * tok, join = ceil(tok / 16.0) * 1800;
+  pieces = 1;
   if (kind == kMxShared) {
-    const double shares = 2 * tiles <= sms ? tiles * fmin(floor(sms / tiles), steps) : sms;
-    return 5000 + ceil(tiles * steps / shares) * step(shares) + 3000 + 50.0 * tok;
+    if (2 * tiles > sms)           // equal shares: a CTA joins pieces at both of its ends
+      return 5000 + ceil(tiles * steps / sms) * step(sms) + 2 * (3000 + join);
+    double best = 0;
+    for (uint32_t p = 2; p <= 16 && p <= steps && p * tiles <= sms; ++p) {
+      const double cost = 5000 + ceil(steps / p) * step(p * tiles) + 3000 + ceil(p / 4.0) * join;
+      if (pieces == 1 || cost < best) {
+        best = cost;
+        pieces = p;
+      }
+    }
+    return pieces == 1 ? 1e30 : best;
   }
   const double waves = floor(tiles / sms), rest = tiles - waves * sms;
+  const double product = waves * (steps * step(sms) + 300) + (rest > 0 ? steps * step(rest) + 300 : 0) + item;
   if (kind == kMxOneLaunch) {
     const double rows = tok < n_rows / slots ? tok : n_rows / slots;
     const double at_once = rows > 4 ? 8 : rows > 2 ? 4 : rows > 1 ? 2 : 1;
-    const double pieces = ceil(rows / at_once) * ceil((double)w.blocks() * at_once / 32);
-    const double quantise = 800 + ceil(pieces / (4 + kMxHelpers)) * 1200;
-    return ceil(tiles / sms) * quantise + waves * (steps * step(sms) + 300) + (rest > 0 ? steps * step(rest) + 300 : 0) +
-           8.0 * tok;
+    const double parts = ceil(rows / at_once) * ceil((double)w.blocks() * at_once / 32);
+    return ceil(tiles / sms) * (800 + ceil(parts / (4 + kMxHelpers)) * 1200) + product;
   }
-  return 5000 + waves * (steps * step(sms) + 300) + (rest > 0 ? steps * step(rest) + 300 : 0) + 8.0 * tok;
+  return 5000 + (kind == kMxPaired ? 2000 : 0) + product;
 }
 
 // Pairs of CTAs that the device runs at a time.
@@ -1151,13 +1192,15 @@ static bool mx_make_plan(const MxShape &w, uint64_t n_rows, bool grouped, MxPlan
                                    g.steps * (t * 128 + (t > 128 ? 2 : 1) * 2ull * kMxChunk) + 4 * kMxStepBytes >
                                        kMaxDynamicSmem - 128 - kMxMiscBytes))
         continue;
-      const double cost = mx_cost(t, slots, w, (double)n_rows, hit, kind == kMxPaired ? n_pairs : sms, kind);
+      uint32_t pieces;
+      const double cost = mx_cost(t, slots, w, (double)n_rows, hit, kind == kMxPaired ? n_pairs : sms, kind, pieces);
       if (best < 0 || cost < best) {
         best = cost;
         tok = t;
         g.split = kind == kMxShared;
         g.pair = kind == kMxPaired;
         g.fused = kind == kMxOneLaunch;
+        g.pieces = pieces;
       }
     }
     if (t >= n_rows) break;
@@ -1438,7 +1481,7 @@ extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t row
   p.steps = g.steps;
   p.blocks = (uint32_t)w.blocks();
   p.x_step_bytes = g.x_step_bytes;
-  p.split = g.split;
+  p.split = g.split ? (g.pieces > 1 ? g.pieces : 4) : 0;
   p.in_block = g.in_block;
   p.pair = g.pair;
   p.x_resident = g.x_resident;

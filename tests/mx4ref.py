@@ -8,8 +8,10 @@ GRID = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float6
 
 
 def quantize(w):
-    """(scale exponents with None-like NaN, values) of a tensor's rows; values in 64 bits."""
+    """The numbers that a tensor's rows become, in 64 bits."""
     v = w.detach().cpu().double()
+    if v.numel() > 1 << 21 and v.dim() > 1:                  # in pieces: the distances take eight times the room
+        return torch.cat([quantize(part) for part in v.split(max(1, v.shape[0] * (1 << 20) // v.numel()))])
     cols = v.shape[-1]
     blocks = -(-cols // 32)
     full = torch.zeros(v.shape[:-1] + (blocks * 32,), dtype=torch.float64)

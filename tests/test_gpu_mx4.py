@@ -187,6 +187,51 @@ def test_linear_gives_the_same_bits_again():
             assert torch.equal(m.linear(h, x), first)
 
 
+@pytest.mark.parametrize("rows,out,inner", [
+    (1, 1200, 4096), (2, 1000, 4000), (3, 300, 8192), (1, 3500, 8192), (7, 513, 5000), (16, 2048, 2048),
+    (24, 140, 16400), (64, 2000, 1024), (200, 4100, 260), (1500, 1030, 288), (1201, 2049, 96), (2600, 520, 1056)])
+def test_linear_every_way_of_running(rows, out, inner):
+    """Few rows, one launch, shared tiles, whole tiles, pairs: the sizes at which each is taken."""
+    check_linear(rand(100, rows, inner), rand(101, out, inner, scale=0.05), rand(102, out) if rows % 2 else None)
+
+
+@pytest.mark.parametrize("rows", (1, 40, 700))
+@pytest.mark.parametrize("a,b", [(1e30, 1e-30), (3e38, 1e-37), (1e-30, 1e30), (1e-39, 1e36), (1e-37, 1e-2),
+                                 (1e36, 1e-39)])
+def test_linear_at_the_ends_of_the_range(rows, a, b):
+    # scales whose product is an ordinary number, and sums that stay in range
+    x = (rand(103, rows, 256, dtype=torch.float32).clamp(-3, 3) / 3 * a).to(BF16)
+    w = (rand(104, 300, 256, dtype=torch.float32).clamp(-3, 3) / 3 * b).to(BF16)
+    check_linear(x, w)
+
+
+def test_linear_outputs_and_inputs_beyond_32_bits():
+    m = neuzip.MX4Manager()
+    w = rand(105, 32768, 64)
+    h = m.write(w.cuda())
+    x = rand(106, 64, 64).cuda().repeat(1100, 1)              # y: 70400 x 32768 elements, over 2^31
+    y = m.linear(h, x)
+    want, bound = mx4ref.product(x[:4].cpu(), w)
+    for r in (0, 64 * 511, 64 * 1023, 64 * 1099):
+        mx4ref.check(y[r:r + 4], want, bound)
+    del y, x
+    w = rand(107, 40, 65536)
+    h = m.write(w.cuda())
+    x = rand(108, 2, 65536).cuda().repeat(16500, 1)           # x: over 2^32 bytes
+    y = m.linear(h, x)
+    want, bound = mx4ref.product(x[:2].cpu(), w)
+    for r in (0, 16382, 32766, 32998):
+        mx4ref.check(y[r:r + 2], want, bound)
+
+
+def test_linear_bias_with_gaps():
+    w, x, b = rand(109, 130, 96), rand(110, 20, 96), rand(111, 260)
+    m = neuzip.MX4Manager()
+    y = m.linear(m.write(w.cuda()), x.cuda(), b.cuda()[::2])
+    want, bound = mx4ref.product(x, w, b[::2])
+    mx4ref.check(y, want, bound)
+
+
 # ------------------------------------------------------------------ grouped
 def check_grouped(x, w, ids, bias=None):
     m = neuzip.MX4Manager()
@@ -218,6 +263,60 @@ def test_grouped_sizes(tokens, k, experts, out, inner, shared):
     x = rand(40, *((tokens, inner) if shared else (tokens, k, inner)))
     check_grouped(x, rand(41, experts, out, inner, scale=0.1), routes(42, tokens, k, experts),
                   rand(43, experts, out) if out % 2 else None)
+
+
+@pytest.mark.parametrize("tokens,k,experts", [(512, 2, 256), (1024, 1, 3), (1025, 1, 3), (205, 5, 257), (129, 8, 256),
+                                              (64, 1, 70), (65, 1, 70), (300, 9, 9), (1, 8, 8), (3000, 1, 2)])
+def test_grouped_limits(tokens, k, experts):
+    """Around the numbers of rows and matrices at which another way of grouping is taken."""
+    check_grouped(rand(112, tokens, 72), rand(113, experts, 24, 72), routes(114, tokens, k, experts))
+
+
+@pytest.mark.parametrize("tokens,k,experts,out,inner", [(1, 2, 4, 600, 8192), (2, 1, 2, 2100, 4096), (30, 4, 16, 400, 1024),
+                                                        (600, 2, 4, 520, 544), (900, 3, 3, 257, 1000)])
+def test_grouped_every_way_of_running(tokens, k, experts, out, inner):
+    check_grouped(rand(115, tokens, inner), rand(116, experts, out, inner, scale=0.05), routes(117, tokens, k, experts),
+                  rand(118, experts, out))
+
+
+def test_grouped_many_rows_without_an_expert():
+    ids = torch.randint(-1, 5, (1400, 3), generator=torch.Generator().manual_seed(119))
+    check_grouped(rand(120, 1400, 100), rand(121, 5, 131, 100), ids)
+    ids[:] = -1
+    check_grouped(rand(122, 1400, 100), rand(121, 5, 131, 100), ids)
+
+
+def test_grouped_numbers_outside_a_large_stack():
+    m = neuzip.MX4Manager()
+    w = rand(123, 3, 20, 64)
+    h = m.write(w.cuda())
+    ids = torch.randint(0, 3, (2000,), generator=torch.Generator().manual_seed(124))
+    ids[7], ids[1999] = 3, -5
+    x = rand(125, 2000, 64)
+    y = m.grouped_linear(h, x.cuda(), ids.cuda()).cpu()
+    assert not y[7].any() and not y[1999].any()
+    for e in range(3):
+        mx4ref.check(y[ids == e], *mx4ref.product(x[ids == e], w[e]))
+    with pytest.raises(_lib.NeuzipError, match="out of range"):
+        m.check()
+    with pytest.raises(ValueError, match="at most"):
+        big = m.write(torch.zeros(8193, 1, 32, dtype=BF16, device="cuda"))
+        m.grouped_linear(big, x[:, :32].cuda(), ids.cuda())
+
+
+def test_grouped_strided_inputs():
+    m = neuzip.MX4Manager()
+    w = rand(126, 5, 40, 96)
+    h = m.write(w.cuda())
+    wide = rand(127, 50, 300)
+    ids = routes(128, 50, 2, 5)
+    for lo in (0, 1, 8, 16):
+        y = m.grouped_linear(h, wide.cuda()[:, lo:lo + 96], ids.cuda().t().contiguous().t()).cpu()
+        for j in range(2):
+            for e in range(5):
+                at = ids[:, j] == e
+                if at.any():
+                    mx4ref.check(y[at, j], *mx4ref.product(wide[at, lo:lo + 96], w[e]))
 
 
 def test_grouped_fp16_and_int32():
@@ -344,6 +443,32 @@ def test_linear_under_autograd():
     assert ((got - dw).abs() <= 2.0 ** -8 * dw.abs() + 8 * 2.0 ** -23 * s).all()
 
 
+def test_linear_gradient_against_differences():
+    """Where inputs are numbers of the format their rounding is the identity: between two such points
+    the layer is linear, and its gradient is the slope."""
+    m = neuzip.MX4Manager()
+    model = m.convert(torch.nn.Sequential(torch.nn.Linear(64, 24, dtype=BF16, bias=False).cuda()))
+    g = torch.Generator().manual_seed(79)
+    points = []
+    for _ in range(2):
+        p = mx4ref.GRID[torch.randint(0, 8, (5, 64), generator=g)] * torch.randint(0, 2, (5, 64), generator=g).mul(2).sub(1)
+        p[:, ::32] = 6                                        # every block has the scale 1
+        points.append(p.to(BF16).cuda())
+    up = torch.randint(-2, 3, (5, 24), generator=g).to(BF16).cuda()
+    x = points[0].clone().requires_grad_()
+    y0 = model(x)
+    y0.backward(up)
+    with torch.no_grad():
+        y1 = model(points[1])
+    step = (points[1] - points[0]).double()
+    slope = (x.grad.double() * step).sum()
+    rise = (up.double() * (y1.detach().double() - y0.detach().double())).sum()
+    # both sides are sums of values rounded to bf16, each off by half a step at most
+    room = 2.0 ** -8 * ((x.grad.double() * step).abs().sum()
+                        + (up.double().abs() * (y1.detach().double().abs() + y0.detach().double().abs())).sum())
+    assert (slope - rise).abs() <= room
+
+
 def test_graph_replay_follows_its_inputs():
     m = neuzip.MX4Manager()
     w, stack = rand(80, 500, 512), rand(81, 6, 130, 512)
@@ -365,6 +490,47 @@ def test_graph_replay_follows_its_inputs():
         want = m.linear(h, x), m.grouped_linear(hs, x, ids)
         for _, a, b in graphs:
             assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
+def test_a_graph_keeps_the_bytes_it_reads():
+    m = neuzip.MX4Manager()
+    w = rand(130, 300, 512)
+    h = m.write(w.cuda())
+    x = rand(131, 20, 512).cuda()
+    want = m.linear(h, x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = m.linear(h, x)
+    for seed in range(4):                    # the handle is written again, and what was freed is reused
+        m.write(rand(132 + seed, 300, 512).cuda(), h)
+        torch.full((300 * 512,), 255, dtype=torch.uint8, device="cuda")
+    graph.replay()
+    assert torch.equal(y, want)
+
+
+def test_threads_share_a_manager():
+    import threading
+    m = neuzip.MX4Manager()
+    ws = [rand(140 + i, 200 + i, 256) for i in range(4)]
+    hs = [m.write(w.cuda()) for w in ws]
+    x = rand(150, 33, 256).cuda()
+    want = [m.linear(h, x) for h in hs]
+    bad = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not torch.equal(m.linear(hs[k], x), want[k]):
+                    bad.append(k)
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_calls_on_two_streams():
