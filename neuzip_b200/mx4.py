@@ -47,6 +47,23 @@ class _Entry:
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
+class _Here:
+    """Nothing to do: the device is the current one already."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(device: torch.device):
+    return _HERE if device.index == _current_device() else torch.cuda.device(device)
+
+
 def _stack(shape: Sequence[int]):
     """How a tensor is stored: three dimensions are a stack of matrices, anything else rows."""
     if len(shape) == 0:
@@ -126,16 +143,20 @@ class MX4Backend:
             raise RuntimeError("Unsupported data type")
         if not tensor.is_cuda:
             tensor = tensor.cuda()
-        source = tensor.detach().contiguous()
-        device = source.get_device()
-        matrices, rows, cols = _stack(source.shape)
-        with torch.cuda.device(device):
-            self._status_of(device)
+        source = tensor if tensor.is_contiguous() else tensor.detach().contiguous()
+        with _on(source.device):
+            device = source.get_device()
+            if device not in self._status:
+                self._status_of(device)
+            shape = source.shape
+            matrices, rows, cols = _stack(shape)
             packed = torch.empty(_stored_bytes(matrices, rows, cols), dtype=torch.uint8, device=source.device)
             stream = torch._C._cuda_getCurrentRawStream(device)
-            _lib.check(self._lib.nz_mx4_quantize(_ptr(source), _DTYPES[tensor.dtype], matrices, rows, cols,
-                                                 _ptr(packed), stream))
-        self._cache[name] = _Entry(tensor.shape, tensor.dtype, matrices, rows, cols, packed, {stream})
+            rc = self._lib.nz_mx4_quantize(source.data_ptr(), _DTYPES[source.dtype], matrices, rows, cols,
+                                           packed.data_ptr(), stream)
+            if rc:
+                _lib.check(rc)
+        self._cache[name] = _Entry(shape, source.dtype, matrices, rows, cols, packed, {stream})
 
     def read(self, name: str) -> torch.Tensor:
         """The stored numbers as a flat tensor of the type that was written."""
@@ -143,12 +164,17 @@ class MX4Backend:
         return self.read_shaped(name, (entry.numel,))
 
     def read_shaped(self, name: str, shape) -> torch.Tensor:
+        """`read` into a tensor of the given shape (one size may be -1)."""
         entry = self._get(name)
-        with torch.cuda.device(entry.device):
-            out = torch.empty(entry.numel, dtype=entry.dtype, device=entry.device).view(tuple(shape))
-            _lib.check(self._lib.nz_mx4_dequantize(
-                _ptr(entry.packed), entry.matrices, entry.rows, entry.cols,
-                _DTYPES[entry.dtype], _ptr(out), self._use(entry)))
+        with _on(entry.device):
+            if shape == entry.shape:
+                out = torch.empty(shape, dtype=entry.dtype, device=entry.device)
+            else:
+                out = torch.empty(entry.numel, dtype=entry.dtype, device=entry.device).view(tuple(shape))
+            rc = self._lib.nz_mx4_dequantize(entry.packed.data_ptr(), entry.matrices, entry.rows, entry.cols,
+                                             _DTYPES[entry.dtype], out.data_ptr(), self._use(entry))
+            if rc:
+                _lib.check(rc)
         return out
 
     def read_many(self, names: Sequence[str]) -> List[torch.Tensor]:
@@ -171,7 +197,7 @@ class MX4Backend:
                 raise ValueError(f"row length {row_len} is not a whole number of stored rows")
             run = row_len // entry.cols
             rows = (rows.unsqueeze(1) * run + torch.arange(run, device=device)).reshape(-1)
-        with torch.cuda.device(device):
+        with _on(device):
             out = torch.empty(rows.numel(), entry.cols, dtype=entry.dtype, device=device)
             _lib.check(self._lib.nz_mx4_gather_rows(
                 _ptr(entry.packed), entry.matrices, entry.rows, entry.cols,
