@@ -17,11 +17,12 @@ mx4_quantize_kernel(const T *__restrict__ in, MxShape s, uint8_t *__restrict__ p
   const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
   const uint32_t halves = 2 * (uint32_t)s.steps(), blocks = (uint32_t)s.blocks();
   const uint32_t tile_groups = (uint32_t)s.row_tiles() * (kMxTileRows / 8);
-  const uint64_t tile_bytes = s.tile_bytes(), total = s.matrices * tile_groups * halves;
-  for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
-    const uint64_t group = w / halves;
-    const uint32_t half = (uint32_t)(w - group * halves), block = half * 4 + (lane >> 3);
-    const uint64_t matrix = group / tile_groups;
+  const uint64_t tile_bytes = s.tile_bytes(), groups = s.matrices * tile_groups;
+  for (MxWalk w((uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5), warps, halves); w.group < groups;
+       w.next()) {
+    const uint64_t group = w.group;
+    const uint32_t half = w.piece, block = half * 4 + (lane >> 3);
+    const uint64_t matrix = s.matrices == 1 ? 0 : group >> 32 ? group / tile_groups : (uint32_t)group / tile_groups;
     const uint32_t row = (uint32_t)(group - matrix * tile_groups) * 8 + (lane & 7u);
     uint32_t v[16], code[4], byte;
     const T *src = in + (matrix * s.rows + row) * s.cols;
@@ -52,8 +53,8 @@ struct MxPlace {
   const uint8_t *codes, *scale;
 };
 __device__ __forceinline__ MxPlace mx_place(const uint8_t *packed, const MxShape &s, uint64_t row, uint32_t block) {
-  const uint64_t matrix = s.matrices == 1 ? 0 : row / s.rows;
-  const uint32_t r = (uint32_t)(row - matrix * s.rows), blocks = (uint32_t)s.blocks(), first = block & ~7u;
+  const uint32_t matrix = s.matrices == 1 ? 0 : (uint32_t)row / (uint32_t)s.rows;    // the stack has < 2^31 rows
+  const uint32_t r = (uint32_t)(row - (uint64_t)matrix * s.rows), blocks = (uint32_t)s.blocks(), first = block & ~7u;
   const uint8_t *step = packed + (matrix * s.row_tiles() + r / kMxTileRows) * s.tile_bytes() +
                         (uint64_t)(block >> 3) * kMxStepBytes;
   const uint32_t held = blocks - first < 8 ? blocks - first : 8;
@@ -85,10 +86,11 @@ mx4_dequantize_kernel(const uint8_t *__restrict__ packed, MxShape s, const int64
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t warps = (uint64_t)gridDim.x * (kMxThreads / 32);
   const uint32_t blocks = (uint32_t)s.blocks(), quads = (blocks + 3) / 4;
-  const uint64_t total = (out_rows + 7) / 8 * quads;
-  for (uint64_t w = (uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
-    const uint64_t group = w / quads, to = group * 8 + (lane & 7u);
-    const uint32_t quad = (uint32_t)(w - group * quads), block = quad * 4 + (lane >> 3);
+  const uint64_t groups = (out_rows + 7) / 8;
+  for (MxWalk w((uint64_t)blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5), warps, quads); w.group < groups;
+       w.next()) {
+    const uint64_t group = w.group, to = group * 8 + (lane & 7u);
+    const uint32_t quad = w.piece, block = quad * 4 + (lane >> 3);
     uint64_t row;
     uint4 code = make_uint4(0, 0, 0, 0);
     uint32_t byte = 0;
@@ -167,7 +169,7 @@ bool mx_dtype(const char *who, int dtype) {
 }
 static unsigned mx_grid(uint64_t warps) {
   const uint64_t blocks = (warps + kMxThreads / 32 - 1) / (kMxThreads / 32);
-  // what is resident at a time: 5 blocks an SM (4096 x 11008: 26.2 us; 8 a grid-stride SM 27.3, 32 28.5)
+  // what is resident at a time: 5 blocks an SM (4096 x 11008: 25.0 us; 4 an SM 27.6, 6 29.6)
   const uint64_t most = (uint64_t)sm_count() * 5;
   return (unsigned)(blocks < most ? blocks : most);
 }

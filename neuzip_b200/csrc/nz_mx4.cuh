@@ -115,6 +115,23 @@ __host__ __device__ __forceinline__ uint32_t mx_scale_offset(uint32_t r, uint32_
   return ((b >> 2) * chunks + (r >> 7)) * kMxChunk + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (b & 3u);
 }
 
+// The items w, w + stride, ... of groups of `per` pieces each, without a 64-bit division for every one
+// (4096 x 11008 is quantised in 25.0 us so and in 26.6 with divisions, 28672 x 8192 in 105 and 110).
+struct MxWalk {
+  uint64_t group, far;
+  uint32_t piece, near, per;
+  __device__ __forceinline__ MxWalk(uint64_t w, uint64_t stride, uint32_t per_)
+      : group(w / per_), far(stride / per_), piece((uint32_t)(w % per_)), near((uint32_t)(stride % per_)), per(per_) {}
+  __device__ __forceinline__ void next() {
+    group += far;
+    piece += near;
+    if (piece >= per) {
+      piece -= per;
+      ++group;
+    }
+  }
+};
+
 // Rows that are not even 16-byte aligned go through shared memory, eight rows of 128 columns a warp:
 // loads and stores of a warp are then runs of a row, and a thread still has a block.
 struct MxTurn {

@@ -517,9 +517,10 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const MxLinearAr
   constexpr uint32_t kAhead = 4;
   const uint32_t apart = p.pair ? p.tok / 2 : p.tok;            // rows of a block of codes
   const uint32_t halves = 2 * p.steps, inputs = p.n_rows / serves;
-  const uint64_t total = (uint64_t)((inputs + 7) / 8) * halves;
-  for (uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (uint64_t)gridDim.x * 8) {
-    const uint32_t group = (uint32_t)(w / halves), half = (uint32_t)(w - (uint64_t)group * halves);
+  const uint32_t groups = (inputs + 7) / 8;
+  for (MxWalk w((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5), (uint64_t)gridDim.x * 8, halves); w.group < groups;
+       w.next()) {
+    const uint32_t group = (uint32_t)w.group, half = w.piece;
     const uint32_t row = group * 8 + (lane & 7u), block = half * 4 + (lane >> 3);
     uint32_t v[16], code[4], byte;
     // where the row goes, known before the row is there
