@@ -37,13 +37,13 @@ struct MxFewArgs {
   uint32_t *status;
 };
 
-// 2^(a + b - 254), the product of the scales of two blocks; exact down to 2^-149, the largest finite
-// power where it would overflow, NaN where either is.
-__device__ __forceinline__ float mx_few_scale(uint32_t a, uint32_t b) {
-  if (a == 255u || b == 255u) return __uint_as_float(0x7FFFFFFFu);
-  const int e = (int)(a + b) - 254 + 127;
-  if (e > 0) return __uint_as_float((uint32_t)(e < 254 ? e : 254) << 23);
-  return e > -23 ? __uint_as_float(0x00800000u >> (1 - e)) : 0.f;
+// The sum of a block's products times 2^(a + b - 254), the scales of the two blocks, added to `to`; NaN where
+// either scale is.  The power may lie far outside fp32 while the product does not (a sum of 1/4 times 2^128, or of
+// a thousand times 2^-150): it is multiplied by halves, and only the sum with `to` rounds.
+__device__ __forceinline__ float mx_few_add(float sum, uint32_t a, uint32_t b, float to) {
+  const int e = (int)(a + b) - 254, h = e >> 1;
+  const float first = __uint_as_float((uint32_t)(h + 127) << 23), second = __uint_as_float((uint32_t)(e - h + 127) << 23);
+  return fmaf(sum * first, a == 255u || b == 255u ? __uint_as_float(0x7FFFFFFFu) : second, to);
 }
 
 __device__ __forceinline__ void mx_few_fma(uint32_t &acc, uint32_t a, uint32_t b) {
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kMxFewWarps * 32, 1) mx4_few_kernel(const MxFe
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const float2 f = mx_few_floats(acc[t][0]), g = mx_few_floats(acc[t][1]);
-        sum[t] = fmaf((f.x + f.y) + (g.x + g.y), mx_few_scale(ws, xs[t * p.blocks + 8 * step + b]), sum[t]);
+        sum[t] = mx_few_add((f.x + f.y) + (g.x + g.y), ws, xs[t * p.blocks + 8 * step + b], sum[t]);
       }
     }
   };

@@ -205,6 +205,20 @@ def test_linear_at_the_ends_of_the_range(rows, a, b):
     check_linear(x, w)
 
 
+@pytest.mark.parametrize("rows", (1, 2, 40, 700))
+@pytest.mark.parametrize("power", (125, 126, 127, 128, 140, -120, -126, -130, -133, -140))
+def test_linear_results_whose_scales_leave_the_range(rows, power):
+    # the largest numbers of the blocks meet zeros; what is left, 1/2 times 1/2 of the scales, is 2^power
+    a = power // 2
+    w, x = torch.zeros(3, 64), torch.zeros(rows, 64)
+    w[:, 0], w[:, 2] = 2.0 ** (a + 3), 2.0 ** a
+    x[:, 1], x[:, 2] = 2.0 ** (power - a + 3), -2.0 ** (power - a)
+    m = neuzip.MX4Manager()
+    y = m.linear(m.write(w.to(BF16).cuda()), x.to(BF16).cuda()).cpu()
+    want = torch.full((rows, 3), -2.0 ** power, dtype=torch.float64).to(BF16)       # infinite, and 0, beyond bf16
+    assert torch.equal(y, want)
+
+
 def test_linear_outputs_and_inputs_beyond_32_bits():
     m = neuzip.MX4Manager()
     w = rand(105, 32768, 64)
