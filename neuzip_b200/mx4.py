@@ -317,9 +317,9 @@ class MX4Backend:
         dtype = {v: k for k, v in _NAMES.items()}.get(blob["dtype"])
         if dtype is None or tuple(blob["stack"]) != stack:
             raise ValueError("checkpoint entry: type or shape does not fit the stored bytes")
-        if blob["packed"].numel() != _stored_bytes(*stack):
+        if blob["packed"].dtype != torch.uint8 or blob["packed"].numel() != _stored_bytes(*stack):
             raise ValueError("checkpoint entry: the stored bytes have the wrong length")
-        packed = blob["packed"].to(device="cuda", dtype=torch.uint8).contiguous()
+        packed = blob["packed"].to(device="cuda", copy=True).contiguous()
         device = packed.get_device()
         self._status_of(device)
         self._cache[name] = _Entry(shape, dtype, *stack, packed,

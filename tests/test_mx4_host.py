@@ -140,7 +140,7 @@ def test_import_refuses_what_does_not_fit():
     blob = {"format": "MXFP4", "dtype": "bfloat16", "shape": (4, 64), "stack": (1, 4, 64),
             "packed": torch.zeros(2 * 2048 + 1024, dtype=torch.uint8)}
     for change in ({"format": "NZR1"}, {"dtype": "float32"}, {"shape": (4, 65)},
-                   {"packed": torch.zeros(5119, dtype=torch.uint8)}):
+                   {"packed": torch.zeros(5119, dtype=torch.uint8)}, {"packed": torch.zeros(5120)}):
         with pytest.raises(ValueError):
             m.import_entry({**blob, **change}, "w")
 
