@@ -146,9 +146,9 @@ __global__ void __launch_bounds__(kMxFewWarps * 32, 1) mx4_few_kernel(const MxFe
   MxFewStep even, odd;
   request(even);
   request(odd);
-  uint32_t turn = 0, count = 0;
+  uint32_t turn = 0, half = 0;
   int64_t have = -1;                           // the row of x in shared memory
-  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x, ++count) {
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
     const uint32_t row = p.experts ? item / strips : 0, strip = item % strips;
     const int64_t matrix = matrix_of(item);
     const uint32_t feature = strip * wide + sub * 32 + lane;
@@ -195,16 +195,18 @@ __global__ void __launch_bounds__(kMxFewWarps * 32, 1) mx4_few_kernel(const MxFe
         ++turn;
       }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) sums[count & 1u][warp][t][lane] = sum[t];
-    // one barrier an item: these sums are written again two items on, behind the next barrier
+    for (int t = 0; t < NT; ++t) sums[half][warp][t][lane] = sum[t];
+    // One barrier for an item with a matrix: these sums are written again two such items on, behind the barrier
+    // of the one between.  Items without a matrix pass no barrier and take no turn.
     __syncthreads();
     for (int t = part; t < NT; t += p.split)
       if (row + t < p.n_rows && feature < p.w.rows) {
         float total = 0.f;
-        for (uint32_t k = 0; k < p.split; ++k) total += sums[count & 1u][sub * p.split + k][t][lane];
+        for (uint32_t k = 0; k < p.split; ++k) total += sums[half][sub * p.split + k][t][lane];
         if (p.bias) total += to_float<T>(((const T *)p.bias)[(uint64_t)matrix * p.w.rows + feature]);
         ((T *)p.y)[(uint64_t)(row + t) * p.w.rows + feature] = from_float<T>(total);
       }
+    half ^= 1u;
   }
 }
 
