@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kMxFewWarps * 32, 1) mx4_few_kernel(const MxFe
   request(even);
   request(odd);
   uint32_t turn = 0, half = 0;
-  int64_t have = -1;                           // the row of x in shared memory
+  int64_t have = -1;                           // the row of x (the first of NT) in shared memory
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
     const uint32_t row = p.experts ? item / strips : 0, strip = item % strips;
     const int64_t matrix = matrix_of(item);
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kMxFewWarps * 32, 1) mx4_few_kernel(const MxFe
       for (uint32_t i = threadIdx.x; i < NT * p.blocks; i += kMxFewWarps * 32) {
         const uint32_t t = i / p.blocks, block = i - t * p.blocks;
         uint32_t v[16], c[4], byte;
-        const T *src = (const T *)p.x + ((uint64_t)have + t) * p.x_stride + (uint64_t)block * kMxBlock;
+        const T *src = (const T *)p.x + (row + t) / p.per_input * p.x_stride + (uint64_t)block * kMxBlock;
         const int64_t left = row + t < p.n_rows ? (int64_t)p.w.cols - (int64_t)block * kMxBlock : 0;
         if (p.wide == 2) mx_load_block<2>(src, left, v);
         else if (p.wide == 1) mx_load_block<1>(src, left, v);

@@ -39,3 +39,29 @@ def test_rows_without_a_matrix_between_rows_of_one_input(missing, out, inner, dt
             m.check()
     else:
         m.check()
+
+
+@pytest.mark.parametrize("n_rows,per_input", [(1, 1), (2, 1), (2, 2), (4, 4), (40, 2), (40, 40), (600, 3), (2600, 2)])
+@pytest.mark.parametrize("out,inner", [(200, 320), (200, 1000), (65, 33)])
+def test_library_rows_that_share_an_input_without_matrix_numbers(n_rows, per_input, out, inner):
+    """`experts` may be null with any `per_input`: row r is x[r / per_input] times the one matrix.  Behind x's
+    own rows lie NaN that no result may see; one row of x needs no stride."""
+    L = _lib.load()
+    m = neuzip.MX4Manager()
+    w = rand(210, out, inner, scale=0.1)
+    h = m.write(w.cuda())
+    inputs = n_rows // per_input
+    x = rand(211, inputs, inner)
+    held = torch.full((inputs + 64, inner), float("nan"), dtype=torch.bfloat16, device="cuda")
+    held[:inputs] = x.cuda()
+    need = int(L.nz_mx4_linear_workspace_bytes(1, out, inner, n_rows, 0))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want, bound = mx4ref.product(x, w)
+    for stride in (inner,) if inputs > 1 else (inner, 0):
+        y = torch.empty(n_rows, out, dtype=torch.bfloat16, device="cuda")
+        _lib.check(L.nz_mx4_linear(m._be.entry(h).packed.data_ptr(), 1, out, inner, _lib.NZ_DTYPE_BF16, held.data_ptr(),
+                                   stride, n_rows, per_input, None, None, y.data_ptr(), ws.data_ptr(), need,
+                                   status.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        mx4ref.check(y, want.repeat_interleave(per_input, 0), bound.repeat_interleave(per_input, 0))
+    assert status.item() == 0
