@@ -37,6 +37,8 @@ class CompressedAdamW:
                  state_dtype: torch.dtype = torch.float32, fused_update: bool = False) -> None:
         params = list(params)
         self.compressed: List[Parameter] = [p for p in params if isinstance(p, Parameter)]
+        for p in self.compressed:
+            self._need_bf16(p.dtype)
         plain = [p for p in params if not isinstance(p, Parameter) and p.requires_grad]
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         self.group = process_group
@@ -60,6 +62,12 @@ class CompressedAdamW:
         if self.world > 1 and overlap_allreduce:
             for p in self.compressed:
                 self._hooks.append(p.register_post_accumulate_grad_hook(self._start_allreduce))
+
+    @staticmethod
+    def _need_bf16(dtype: torch.dtype) -> None:
+        # the step's kernel takes the weight's bits as bf16
+        if dtype != torch.bfloat16:
+            raise TypeError(f"CompressedAdamW updates bf16 weights, got {dtype}")
 
     # gradient of a compressed weight is ready: start summing it over the ranks
     def _start_allreduce(self, p: Parameter) -> None:
@@ -132,6 +140,7 @@ class CompressedAdamW:
                 p.grad = None
                 continue
             w = p()                                                    # decode (bf16, contiguous)
+            self._need_bf16(w.dtype)               # the handle may have been imported with another type
             self._lib_mod.check(self._lib.nz_adamw_bf16(
                 w.data_ptr(), g.data_ptr(), st["m"].data_ptr(), st["v"].data_ptr(), w.numel(),
                 int(self.state_dtype == torch.bfloat16), self.lr, b1, b2, self.eps,
