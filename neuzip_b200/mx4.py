@@ -83,6 +83,20 @@ def _workspace_bytes(device: int, matrices: int, rows: int, cols: int, n_rows: i
     return int(_lib.load().nz_mx4_linear_workspace_bytes(matrices, rows, cols, n_rows, grouped))
 
 
+class _TrainedBias(torch.autograd.Function):
+    """A product of inputs that need no gradient and a frozen matrix, whose bias is trained: the bias is
+    still added before the one rounding."""
+
+    @staticmethod
+    def forward(ctx, bias, product, entry, x, input):
+        ctx.shape = bias.shape
+        return product(entry, x, input, bias)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        return grad_output.reshape(-1, grad_output.shape[-1]).sum(0).reshape(ctx.shape), None, None, None, None
+
+
 class MX4Backend:
     """`read / write / size / linear / linear_without_bias / split` and the extras of the codec
     backends, on 4-bit storage."""
@@ -213,11 +227,18 @@ class MX4Backend:
     def linear(self, name: str, input: torch.Tensor, shape: Sequence[int],
                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``q(input) @ q(W)^T (+ bias)``: the inputs are quantised like the weights, sums are
-        fp32, the result is rounded once to the type of `input`."""
+        fp32, the result is rounded once to the type of `input`.  Differentiable in `bias` alone;
+        inputs that need a gradient are refused (``nn.Linear`` takes them)."""
         entry = self._get(name)
         if len(shape) != 2 or entry.matrices != 1 or shape[1] != entry.cols or shape[0] != entry.rows:
             raise ValueError(f"linear needs a matrix, got a tensor of shape {tuple(shape)}")
         x = self._checked_input(entry, input, bias)
+        if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+            return _TrainedBias.apply(bias, self._dense, entry, x, input)
+        return self._dense(entry, x, input, bias)
+
+    def _dense(self, entry: _Entry, x: torch.Tensor, input: torch.Tensor,
+               bias: Optional[torch.Tensor]) -> torch.Tensor:
         y = input.new_empty((*input.shape[:-1], entry.rows))
         return self._launch(entry, x, x.shape[0], 1, None, bias, y)
 
@@ -247,6 +268,9 @@ class MX4Backend:
                                  f"{tuple(experts.shape)}")
             per_input = int(experts.shape[-1])
         x = self._checked_input(entry, input, bias)
+        if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("grouped_linear has no gradient for its bias: detach it, or call under "
+                               "torch.no_grad()")
         ids = (experts if experts.dtype == torch.int64 else experts.long()).contiguous()
         y = input.new_empty((*experts.shape, entry.rows))
         return self._launch(entry, x, ids.numel(), per_input, ids, bias, y)
@@ -266,9 +290,9 @@ class MX4Backend:
                                  or bias.numel() != entry.matrices * entry.rows):
             raise ValueError(f"bias must be {entry.matrices * entry.rows} numbers of type "
                              f"{_NAMES[input.dtype]} on {input.device}")
-        if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
-            raise RuntimeError("products with 4-bit weights have no gradient here: use nn.Linear, or "
-                               "call under torch.no_grad()")
+        if input.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("a manager's products with 4-bit weights have no gradient for their inputs: use "
+                               "nn.Linear for one matrix, or call under torch.no_grad()")
         x = input if len(shape) == 2 else input.reshape(-1, entry.cols)
         row, element = x.stride()
         if element != 1 or row < entry.cols:

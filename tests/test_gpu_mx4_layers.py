@@ -1,0 +1,58 @@
+"""Layers on 4-bit storage as training and autocast use them (definition in 64 bits: tests/mx4ref.py)."""
+import pytest
+import torch
+
+import neuzip
+from tests import mx4ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def rand(seed, *shape, dtype=BF16, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def layer(out, inner, dtype=BF16, seed=300):
+    """(layer on 4-bit storage, its matrix and vector before conversion)"""
+    lin = torch.nn.Linear(inner, out, dtype=dtype)
+    with torch.no_grad():
+        lin.weight.copy_(rand(seed, out, inner, dtype=dtype, scale=0.1))
+        lin.bias.copy_(rand(seed + 1, out, dtype=dtype))
+    w, b = lin.weight.detach().clone(), lin.bias.detach().clone()
+    return neuzip.MX4Manager().convert(torch.nn.Sequential(lin.cuda()))[0], w, b
+
+
+@pytest.mark.parametrize("rows", ((1,), (3, 7), (0,)))
+def test_a_bias_trains_over_a_frozen_matrix(rows):
+    lin, w, b = layer(40, 96)
+    lin._p.requires_grad_(False)
+    x, g = rand(302, *rows, 96), rand(303, *rows, 40)
+    y = lin(x.cuda())
+    mx4ref.check(y.view(-1, 40), *mx4ref.product(x.view(-1, 96), w, b))
+    y.backward(g.cuda())
+    # a sum of n terms in fp32 and one rounding to bf16, half a step
+    terms = g.double().view(-1, 40)
+    want = terms.sum(0)
+    room = 2.0 ** -8 * want.abs() + max(1, len(terms)) * 2.0 ** -23 * terms.abs().sum(0) * (1 + 2.0 ** -8)
+    assert ((lin.bias.grad.cpu().double() - want).abs() <= room).all()
+    assert lin._p._gradient is None and lin._p.grad is None
+    # linear in the bias: between two points of it the results rise by the slope, up to both results' bounds
+    with torch.no_grad():
+        lin.bias += 1
+        again = lin(x.cuda()).cpu().double().view(-1, 40)
+    later = lin.bias.detach().cpu()
+    first, second = mx4ref.product(x.view(-1, 96), w, b)[1], mx4ref.product(x.view(-1, 96), w, later)[1]
+    rise = (terms * (again - y.detach().cpu().double().view(-1, 40))).sum()
+    assert (rise - (want * (later.double() - b.double())).sum()).abs() <= (terms.abs() * (first + second)).sum()
+
+
+def test_a_result_with_a_trained_bias_may_be_changed_in_place():
+    lin, _, _ = layer(40, 96)
+    lin._p.requires_grad_(False)
+    y = lin(rand(304, 5, 96).cuda())
+    y.mul_(2)
+    y.sum().backward()
+    assert torch.equal(lin.bias.grad.cpu(), torch.full((40,), 10, dtype=BF16))
