@@ -83,6 +83,13 @@ def _workspace_bytes(device: int, matrices: int, rows: int, cols: int, n_rows: i
     return int(_lib.load().nz_mx4_linear_workspace_bytes(matrices, rows, cols, n_rows, grouped))
 
 
+def _in_autocast_type(tensor: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """What ``functional.linear`` makes of an argument under autocast."""
+    if tensor is None or not tensor.is_floating_point() or tensor.dtype == torch.float64:
+        return tensor
+    return tensor.to(torch.get_autocast_dtype("cuda"))
+
+
 class _TrainedBias(torch.autograd.Function):
     """A product of inputs that need no gradient and a frozen matrix, whose bias is trained: the bias is
     still added before the one rounding."""
@@ -227,11 +234,14 @@ class MX4Backend:
     def linear(self, name: str, input: torch.Tensor, shape: Sequence[int],
                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``q(input) @ q(W)^T (+ bias)``: the inputs are quantised like the weights, sums are
-        fp32, the result is rounded once to the type of `input`.  Differentiable in `bias` alone;
-        inputs that need a gradient are refused (``nn.Linear`` takes them)."""
+        fp32, the result is rounded once to the type of `input` (under autocast, of autocast).
+        Differentiable in `bias` alone; inputs that need a gradient are refused (``nn.Linear``
+        takes them)."""
         entry = self._get(name)
         if len(shape) != 2 or entry.matrices != 1 or shape[1] != entry.cols or shape[0] != entry.rows:
             raise ValueError(f"linear needs a matrix, got a tensor of shape {tuple(shape)}")
+        if torch.is_autocast_enabled():
+            input, bias = _in_autocast_type(input), _in_autocast_type(bias)
         x = self._checked_input(entry, input, bias)
         if bias is not None and bias.requires_grad and torch.is_grad_enabled():
             return _TrainedBias.apply(bias, self._dense, entry, x, input)
@@ -267,6 +277,8 @@ class MX4Backend:
                 raise ValueError(f"inputs of shape {tuple(input.shape)} do not match experts of shape "
                                  f"{tuple(experts.shape)}")
             per_input = int(experts.shape[-1])
+        if torch.is_autocast_enabled():
+            input, bias = _in_autocast_type(input), _in_autocast_type(bias)
         x = self._checked_input(entry, input, bias)
         if bias is not None and bias.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("grouped_linear has no gradient for its bias: detach it, or call under "

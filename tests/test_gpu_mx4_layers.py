@@ -56,3 +56,34 @@ def test_a_result_with_a_trained_bias_may_be_changed_in_place():
     y.mul_(2)
     y.sum().backward()
     assert torch.equal(lin.bias.grad.cpu(), torch.full((40,), 10, dtype=BF16))
+
+
+@pytest.mark.parametrize("to", (BF16, FP16))
+@pytest.mark.parametrize("needs", ("nothing", "inputs", "bias"))
+def test_layers_under_autocast(to, needs):
+    """fp32 inputs and an fp32 bias over a bf16 matrix, as functional.linear takes them under autocast."""
+    lin, w, _ = layer(40, 96)
+    lin._p.requires_grad_(needs == "inputs")
+    b = rand(310, 40, dtype=torch.float32)
+    lin.bias = torch.nn.Parameter(b.cuda(), requires_grad=needs != "nothing")
+    x = rand(311, 9, 96, dtype=torch.float32)
+    xd = x.cuda().requires_grad_(needs == "inputs")
+    with torch.autocast("cuda", dtype=to):
+        y = lin(xd)
+    assert y.dtype == to
+    mx4ref.check(y, *mx4ref.product(x.to(to), w, b.to(to)))
+    if needs == "bias":
+        y.sum().backward()
+        assert torch.equal(lin.bias.grad.cpu(), torch.full((40,), 9.0))
+
+
+@pytest.mark.parametrize("to", (BF16, FP16))
+def test_experts_under_autocast(to):
+    w, b = rand(312, 3, 40, 96, scale=0.1), rand(313, 3, 40, dtype=torch.float32)
+    experts = neuzip.nn.Experts(neuzip.MX4Manager(), w.cuda(), b.cuda())
+    x, ids = rand(314, 3, 96, dtype=torch.float32), torch.arange(3)
+    with torch.autocast("cuda", dtype=to):
+        y = experts(x.cuda(), ids.cuda())
+    assert y.dtype == to
+    for e in range(3):
+        mx4ref.check(y[e:e + 1], *mx4ref.product(x[e:e + 1].to(to), w[e], b[e].to(to)))

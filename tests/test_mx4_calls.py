@@ -47,3 +47,40 @@ def test_the_bias_of_a_stack_has_no_gradient(at_launch):
     with torch.no_grad():
         assert m.grouped_linear("w", x, ids, bias).shape == (5, 2, 32)
     assert m.grouped_linear("w", x, ids, bias.detach()).shape == (5, 2, 32)
+
+
+@pytest.fixture
+def autocast():
+    """Autocast as on a machine with a GPU (torch.autocast switches itself off without one)."""
+    on, dtype = torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda")
+
+    def begin(to):
+        torch.set_autocast_enabled("cuda", True)
+        torch.set_autocast_dtype("cuda", to)
+    yield begin
+    torch.set_autocast_enabled("cuda", on)
+    torch.set_autocast_dtype("cuda", dtype)
+
+
+@pytest.mark.parametrize("to", (BF16, torch.float16))
+@pytest.mark.parametrize("x_type", (torch.float32, BF16, torch.float16))
+@pytest.mark.parametrize("bias_type", (torch.float32, BF16, torch.float16, None))
+def test_autocast_takes_inputs_and_bias_to_its_type(at_launch, autocast, to, x_type, bias_type):
+    autocast(to)
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    bias = [None, None] if bias_type is None else [torch.ones(32, dtype=bias_type), torch.ones(4, 32, dtype=bias_type)]
+    assert manager_with((32, 64)).linear("w", torch.ones(2, 64, dtype=x_type), bias[0]).dtype == to
+    assert manager_with((4, 32, 64)).grouped_linear("w", torch.ones(2, 64, dtype=x_type), ids, bias[1]).dtype == to
+    for x, b, y in at_launch:
+        assert x.dtype == to and y.dtype == to and (b is None or b.dtype == to)
+
+
+def test_autocast_leaves_other_types_refused(at_launch, autocast):
+    autocast(BF16)
+    for dtype in (torch.float64, torch.int32):
+        with pytest.raises(RuntimeError, match="Unsupported data type"):
+            manager_with((32, 64)).linear("w", torch.ones(2, 64, dtype=dtype))
+    x = torch.ones(2, 64)
+    bias = torch.zeros(32, requires_grad=True)
+    manager_with((32, 64)).linear("w", x, bias).sum().backward()
+    assert bias.grad.dtype == torch.float32 and torch.equal(bias.grad, torch.full((32,), 2.0))
