@@ -26,7 +26,14 @@ class CompressedLinear(torch.autograd.Function):
         x2d = inputs.reshape(-1, inputs.shape[-1])
         g2d = grad_output.reshape(-1, grad_output.shape[-1])
         weight = _p()
-        grad_inputs = torch.mm(g2d, weight).reshape(inputs.shape).to(ctx._inputs_dtype)
+        if weight.dtype == g2d.dtype:
+            grad_inputs = torch.mm(g2d, weight)
+        else:
+            # fp16 inputs of a bf16 weight or the other way round (managers that multiply the stored form
+            # take them): neither type holds the other, fp32 holds both
+            wide = torch.promote_types(weight.dtype, g2d.dtype)
+            grad_inputs = torch.mm(g2d.to(wide), weight.to(wide))
+        grad_inputs = grad_inputs.reshape(inputs.shape).to(ctx._inputs_dtype)
         del weight
         grad_weight = torch.mm(g2d.t(), x2d)
         if _p._gradient is None:

@@ -87,3 +87,27 @@ def test_experts_under_autocast(to):
     assert y.dtype == to
     for e in range(3):
         mx4ref.check(y[e:e + 1], *mx4ref.product(x[e:e + 1].to(to), w[e], b[e].to(to)))
+
+
+@pytest.mark.parametrize("wide", (True, False))
+@pytest.mark.parametrize("x_type,w_type", [(FP16, BF16), (BF16, FP16), (BF16, BF16), (FP16, FP16)])
+def test_gradients_of_mixed_types(x_type, w_type, wide):
+    """Inputs and matrix of different 16-bit types; a bf16 matrix beyond fp16's range (`wide`) with gradients that
+    bring the results back into it."""
+    lin, w, _ = layer(40, 96, dtype=w_type)
+    scale = 2.0 ** 20 if wide and w_type == BF16 else 1.0
+    lin.manager.write((w * scale).cuda(), lin._p._handle)
+    wq = mx4ref.quantize(w * scale)
+    lin.bias = None
+    x = rand(320, 8, 96, dtype=x_type, scale=2.0 ** -12 if scale > 1 else 1.0)
+    g = rand(321, 8, 40, dtype=x_type, scale=2.0 ** -12 if scale > 1 else 1.0)
+    xd = x.cuda().requires_grad_()
+    y = lin(xd)
+    mx4ref.check(y, *mx4ref.product(x, w * scale))
+    y.backward(g.cuda())
+    half = torch.finfo(x_type).eps / 2
+    # sums of n products in fp32, one rounding to the type of x and its smallest numbers
+    for got, a, b in ((xd.grad, g.double(), wq), (lin._p._gradient, g.double().t(), x.double())):
+        want, sums = a @ b, a.shape[1] * 2.0 ** -23 * (a.abs() @ b.abs())
+        room = sums + half * (want.abs() + sums) + torch.finfo(x_type).smallest_normal * half
+        assert got.dtype == x_type and ((got.cpu().double() - want).abs() <= room).all()
