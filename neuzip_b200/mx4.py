@@ -17,6 +17,7 @@ from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .backend import _ptr
@@ -81,6 +82,12 @@ def _stored_bytes(matrices: int, rows: int, cols: int) -> int:
 @functools.lru_cache(maxsize=2048)
 def _workspace_bytes(device: int, matrices: int, rows: int, cols: int, n_rows: int, grouped: bool) -> int:
     return int(_lib.load().nz_mx4_linear_workspace_bytes(matrices, rows, cols, n_rows, grouped))
+
+
+def _has_tangent(tensor: Optional[torch.Tensor]) -> bool:
+    # outside every dual_level there is nothing to unpack (which takes 0.4 us)
+    return (tensor is not None and getattr(forward_ad, "_current_level", 0) >= 0
+            and forward_ad.unpack_dual(tensor).tangent is not None)
 
 
 def _in_autocast_type(tensor: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -305,6 +312,8 @@ class MX4Backend:
         if input.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("a manager's products with 4-bit weights have no gradient for their inputs: use "
                                "nn.Linear for one matrix, or call under torch.no_grad()")
+        if _has_tangent(input) or _has_tangent(bias):
+            raise NotImplementedError("products with 4-bit weights have no forward-mode derivative")
         x = input if len(shape) == 2 else input.reshape(-1, entry.cols)
         row, element = x.stride()
         if element != 1 or row < entry.cols:

@@ -84,3 +84,17 @@ def test_autocast_leaves_other_types_refused(at_launch, autocast):
     bias = torch.zeros(32, requires_grad=True)
     manager_with((32, 64)).linear("w", x, bias).sum().backward()
     assert bias.grad.dtype == torch.float32 and torch.equal(bias.grad, torch.full((32,), 2.0))
+
+
+def test_forward_mode_derivatives_are_refused(at_launch):
+    from torch.autograd import forward_ad
+    m, stack = manager_with((32, 64)), manager_with((4, 32, 64))
+    x, bias, ids = torch.zeros(2, 64, dtype=BF16), torch.zeros(32, dtype=BF16), torch.zeros(2, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: m.linear("w", dual), lambda: stack.grouped_linear("w", dual, ids),
+                     lambda: m.linear("w", x, forward_ad.make_dual(bias, torch.ones_like(bias)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert m.linear("w", x, bias).shape == (2, 32)
+    assert not forward_ad.unpack_dual(m.linear("w", x, bias)).tangent
