@@ -249,7 +249,7 @@ class MX4Backend:
             raise ValueError(f"linear needs a matrix, got a tensor of shape {tuple(shape)}")
         if torch.is_autocast_enabled():
             input, bias = _in_autocast_type(input), _in_autocast_type(bias)
-        x = self._checked_input(entry, input, bias)
+        x = self._checked_input(entry, input, bias, (entry.rows,))
         if bias is not None and bias.requires_grad and torch.is_grad_enabled():
             return _TrainedBias.apply(bias, self._dense, entry, x, input)
         return self._dense(entry, x, input, bias)
@@ -267,7 +267,7 @@ class MX4Backend:
         """Row ``r`` of the result is ``q(input[r]) @ q(W[experts[r]])^T (+ bias[experts[r]])`` for a
         stack ``W`` of matrices.  `experts` is an integer tensor; `input` has its shape and one
         more dimension, or lacks its last one, and then every input row goes to all the
-        experts named for it: ``[T, k]`` experts and ``[T, in]`` inputs give ``[T, k, out]``.
+        experts named for it (`bias` is ``[E, out]``): ``[T, k]`` experts and ``[T, in]`` inputs give ``[T, k, out]``.
         -1 means no expert and gives a row of zeros; other numbers outside the stack too, and
         they raise at the next ``check()``.  Nothing synchronises with the host."""
         entry = self._get(name)
@@ -286,7 +286,7 @@ class MX4Backend:
             per_input = int(experts.shape[-1])
         if torch.is_autocast_enabled():
             input, bias = _in_autocast_type(input), _in_autocast_type(bias)
-        x = self._checked_input(entry, input, bias)
+        x = self._checked_input(entry, input, bias, (entry.matrices, entry.rows))
         if bias is not None and bias.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("grouped_linear has no gradient for its bias: detach it, or call under "
                                "torch.no_grad()")
@@ -295,7 +295,7 @@ class MX4Backend:
         return self._launch(entry, x, ids.numel(), per_input, ids, bias, y)
 
     def _checked_input(self, entry: _Entry, input: torch.Tensor,
-                       bias: Optional[torch.Tensor]) -> torch.Tensor:
+                       bias: Optional[torch.Tensor], bias_shape) -> torch.Tensor:
         """`input` as rows one element apart inside, after the checks the products share."""
         if input.dtype not in _DTYPES:
             raise RuntimeError("Unsupported data type")
@@ -305,10 +305,13 @@ class MX4Backend:
                              f"{tuple(entry.shape)}")
         if input.device != entry.device:
             raise ValueError(f"inputs are on {input.device}, the weights on {entry.device}")
-        if bias is not None and (bias.dtype != input.dtype or bias.device != entry.device
-                                 or bias.numel() != entry.matrices * entry.rows):
-            raise ValueError(f"bias must be {entry.matrices * entry.rows} numbers of type "
-                             f"{_NAMES[input.dtype]} on {input.device}")
+        if bias is not None:
+            if bias.dtype != input.dtype or bias.device != entry.device:
+                raise ValueError(f"bias must be of type {_NAMES[input.dtype]} on {entry.device}, got "
+                                 f"{bias.dtype} on {bias.device}")
+            # a vector's numbers have one order whatever its shape, those of a stack do not
+            if bias.shape != bias_shape and (len(bias_shape) > 1 or bias.numel() != entry.rows):
+                raise ValueError(f"bias must have the shape {bias_shape}, got {tuple(bias.shape)}")
         if input.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("a manager's products with 4-bit weights have no gradient for their inputs: use "
                                "nn.Linear for one matrix, or call under torch.no_grad()")

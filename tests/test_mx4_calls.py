@@ -98,3 +98,17 @@ def test_forward_mode_derivatives_are_refused(at_launch):
                 call()
         assert m.linear("w", x, bias).shape == (2, 32)
     assert not forward_ad.unpack_dual(m.linear("w", x, bias)).tangent
+
+
+def test_the_bias_of_a_stack_has_a_row_for_every_matrix(at_launch):
+    m, x, ids = manager_with((4, 32, 64)), torch.zeros(5, 64, dtype=BF16), torch.zeros(5, 2, dtype=torch.int64)
+    for shape in ((32, 4), (4 * 32,), (4, 32, 1), (1, 4, 32), (2, 64), (32,)):
+        with pytest.raises(ValueError, match="shape"):
+            m.grouped_linear("w", x, ids, torch.zeros(shape, dtype=BF16))
+    assert m.grouped_linear("w", x, ids, torch.zeros(32, 4, dtype=BF16).t()).shape == (5, 2, 32)
+    one = manager_with((32, 64))
+    for shape in ((32,), (1, 32), (32, 1)):
+        assert one.linear("w", x, torch.zeros(shape, dtype=BF16)).shape == (5, 32)
+    for shape in ((33,), (2, 32), (), (0,)):
+        with pytest.raises(ValueError, match="shape"):
+            one.linear("w", x, torch.zeros(shape, dtype=BF16))
