@@ -245,3 +245,14 @@ class MX4Manager(Manager):
         holds a stack of matrices ``[E, out, in]`` (and `bias` ``[E, out]``): ``[T, k]`` expert
         numbers and ``[T, in]`` or ``[T, k, in]`` inputs give ``[T, k, out]``; -1 gives zeros."""
         return self._be.grouped_linear(handle, inputs, experts, bias)
+
+    def captured_bytes(self) -> int:
+        """Stored bytes kept only because a captured CUDA graph reads them (the handle has been
+        written again or erased since); not part of `total_size`."""
+        return self._be.captured_bytes()
+
+    def release_captured(self) -> None:
+        """Give up what is kept for captured CUDA graphs, once those graphs are gone or read only
+        handles that stay as they are.  A manager cannot see a graph's end: until this call it
+        keeps every tensor that a capture has read."""
+        self._be.release_captured()

@@ -155,13 +155,27 @@ class MX4Backend:
         the allocator does not hand the entry's memory out while that stream may read it."""
         stream = torch._C._cuda_getCurrentRawStream(entry.device.index)
         if torch._C._cuda_isCurrentStreamCapturing():
-            # the graph reads these bytes at every replay, whatever becomes of the handle
+            # the graph reads these bytes at every replay, whatever becomes of the handle; its end is not
+            # known here, see release_captured
             self._captured[entry.packed.data_ptr()] = entry.packed
         if stream not in entry.streams:
             current = torch.cuda.current_stream(entry.device)
             entry.packed.record_stream(current)
             entry.streams.add(stream)
         return stream
+
+    def captured_bytes(self) -> int:
+        """Stored bytes that are kept for captured graphs alone: their handle has been written
+        again or erased since.  `size` does not count them."""
+        held = {entry.packed.data_ptr() for entry in self._cache.values()}
+        return sum(packed.numel() for at, packed in self._captured.items() if at not in held)
+
+    def release_captured(self) -> None:
+        """Keep nothing more for the graphs that have been captured so far: those that read a handle
+        must not be replayed after it is written again or erased.  Waits for the work under way."""
+        for device in {packed.device for packed in self._captured.values() if packed.is_cuda}:
+            torch.cuda.synchronize(device)
+        self._captured.clear()
 
     # -- the six methods of the extension class ----------------------------
     def write(self, name: str, tensor: torch.Tensor) -> None:

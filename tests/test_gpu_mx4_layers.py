@@ -111,3 +111,27 @@ def test_gradients_of_mixed_types(x_type, w_type, wide):
         want, sums = a @ b, a.shape[1] * 2.0 ** -23 * (a.abs() @ b.abs())
         room = sums + half * (want.abs() + sums) + torch.finfo(x_type).smallest_normal * half
         assert got.dtype == x_type and ((got.cpu().double() - want).abs() <= room).all()
+
+
+def test_bytes_of_captured_graphs_can_be_given_back():
+    m = neuzip.MX4Manager()
+    h = m.write(rand(330, 1024, 1024).cuda())
+    x = rand(331, 20, 1024).cuda()
+    m.linear(h, x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = m.linear(h, x)
+    size = m.size(h)
+    assert m.captured_bytes() == 0
+    m.write(rand(332, 1024, 1024).cuda(), h)
+    assert m.captured_bytes() == size
+    graph.replay()
+    want = y.clone()
+    assert not torch.equal(m.linear(h, x), want)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    graph.reset()
+    m.release_captured()
+    assert m.captured_bytes() == 0 and torch.cuda.memory_allocated() <= before - size
+    m.check()

@@ -112,3 +112,18 @@ def test_the_bias_of_a_stack_has_a_row_for_every_matrix(at_launch):
     for shape in ((33,), (2, 32), (), (0,)):
         with pytest.raises(ValueError, match="shape"):
             one.linear("w", x, torch.zeros(shape, dtype=BF16))
+
+
+def test_bytes_kept_for_captured_graphs_are_counted_and_released():
+    m = manager_with((128, 32))
+    size = m.size("w")
+    entry = m._be.entry("w")
+    assert m.captured_bytes() == 0
+    m._be._captured[entry.packed.data_ptr()] = entry.packed            # as a capture does
+    assert m.captured_bytes() == 0                                     # the handle holds them too
+    m._be._cache["w"] = manager_with((128, 32))._be.entry("w")         # written again
+    assert m.captured_bytes() == size and m.total_size() == size
+    m._be.erase("w")
+    assert m.captured_bytes() == size
+    m.release_captured()
+    assert m.captured_bytes() == 0 and not m._be._captured
