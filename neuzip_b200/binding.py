@@ -231,6 +231,8 @@ class MX4Manager(Manager):
     :class:`Manager`; bf16 and fp16 tensors; `read` returns the stored numbers in the type that
     was written.  Not in the reference."""
 
+    keeps_devices = True      # a tensor stays on the GPU it was written from; `import_entry` takes one
+
     def __init__(self) -> None:
         from .mx4 import MX4Backend
         self._be = MX4Backend()
@@ -245,6 +247,15 @@ class MX4Manager(Manager):
         holds a stack of matrices ``[E, out, in]`` (and `bias` ``[E, out]``): ``[T, k]`` expert
         numbers and ``[T, in]`` or ``[T, k, in]`` inputs give ``[T, k, out]``; -1 gives zeros."""
         return self._be.grouped_linear(handle, inputs, experts, bias)
+
+    def import_entry(self, blob: dict, handle: Optional[str] = None, device=None) -> str:
+        """As in :class:`Manager`; `device` is the GPU that takes the bytes (default: the one that
+        holds `handle` already, else the current one)."""
+        if handle is None:
+            handle = str(len(self.meta_dict))
+        self.meta_dict[handle] = torch.Size(blob["shape"])
+        self._be.import_entry(handle, blob, device)
+        return handle
 
     def captured_bytes(self) -> int:
         """Stored bytes kept only because a captured CUDA graph reads them (the handle has been

@@ -370,8 +370,17 @@ class MX4Backend:
         return {"format": "MXFP4", "dtype": _NAMES[e.dtype], "stack": (e.matrices, e.rows, e.cols),
                 "packed": e.packed.cpu()}
 
-    def import_entry(self, name: str, blob: dict) -> None:
-        """Inverse of `export_entry`: the stored bytes go straight to the GPU."""
+    def _import_device(self, name: str, device) -> torch.device:
+        """The GPU asked for, else the one that holds `name` already, else the current one."""
+        device = None if device is None else torch.device(device)
+        if device is None or device.type != "cuda":
+            held = self._cache.get(name)
+            device = torch.device("cuda") if held is None else held.device
+        return device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
+
+    def import_entry(self, name: str, blob: dict, device=None) -> None:
+        """Inverse of `export_entry`: the stored bytes go straight to `device`, a GPU; by default to
+        the one that holds the entry they replace, or the current one."""
         if blob.get("format") != "MXFP4":
             raise ValueError(f"checkpoint entry does not match this manager (format {blob.get('format')!r})")
         shape = torch.Size(blob["shape"])
@@ -381,11 +390,12 @@ class MX4Backend:
             raise ValueError("checkpoint entry: type or shape does not fit the stored bytes")
         if blob["packed"].dtype != torch.uint8 or blob["packed"].numel() != _stored_bytes(*stack):
             raise ValueError("checkpoint entry: the stored bytes have the wrong length")
-        packed = blob["packed"].to(device="cuda", copy=True).contiguous()
-        device = packed.get_device()
-        self._status_of(device)
-        self._cache[name] = _Entry(shape, dtype, *stack, packed,
-                                   {torch._C._cuda_getCurrentRawStream(device)})
+        device = self._import_device(name, device)
+        with _on(device):
+            packed = blob["packed"].to(device=device, copy=True).contiguous()
+            self._status_of(device.index)
+            self._cache[name] = _Entry(shape, dtype, *stack, packed,
+                                       {torch._C._cuda_getCurrentRawStream(device.index)})
 
     # -- extras -----------------------------------------------------------
     def erase(self, name: str) -> None:

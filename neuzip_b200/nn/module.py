@@ -32,7 +32,10 @@ class Parameter(torch.nn.Parameter):
         self._manager = manager
         self._shape = torch.Size(blob["shape"])
         self._gradient = None
-        self._handle = manager.import_entry(blob)
+        if getattr(manager, "keeps_devices", False):
+            self._handle = manager.import_entry(blob, device=device)
+        else:
+            self._handle = manager.import_entry(blob)
         self._staged = None
         self._stage_tag = None
         return self

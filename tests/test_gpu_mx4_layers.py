@@ -135,3 +135,21 @@ def test_bytes_of_captured_graphs_can_be_given_back():
     m.release_captured()
     assert m.captured_bytes() == 0 and torch.cuda.memory_allocated() <= before - size
     m.check()
+
+
+def test_a_checkpoint_is_loaded_onto_the_devices_of_its_layers():
+    m = neuzip.MX4Manager()
+    w = rand(340, 24, 64)
+    h = m.write(w.cuda())
+    blob = m.export_entry(h)
+    here = torch.device("cuda", torch.cuda.current_device())
+    for name, device in ((h, None), ("a", None), ("b", "cuda"), ("c", here), ("d", "cuda:%d" % here.index)):
+        m.import_entry(blob, name, device)
+        assert m._be.entry(name).device == here
+        assert torch.equal(m.read(name).cpu().double(), mx4ref.quantize(w))
+    if torch.cuda.device_count() > 1:
+        m.import_entry(blob, "e", "cuda:1")
+        m.import_entry(blob, "e")
+        x = rand(341, 3, 64)
+        mx4ref.check(m.linear("e", x.to("cuda:1")), *mx4ref.product(x, w))
+    m.check()

@@ -127,3 +127,36 @@ def test_bytes_kept_for_captured_graphs_are_counted_and_released():
     assert m.captured_bytes() == size
     m.release_captured()
     assert m.captured_bytes() == 0 and not m._be._captured
+
+
+def blob_of(shape=(4, 64), dtype="bfloat16"):
+    from neuzip_b200 import _lib
+    from neuzip_b200.mx4 import _stack
+    stack = _stack(shape)
+    return {"format": "MXFP4", "dtype": dtype, "shape": shape, "stack": stack,
+            "packed": torch.zeros(int(_lib.load().nz_mx4_bytes(*stack)), dtype=torch.uint8)}
+
+
+def test_imported_bytes_go_to_the_device_of_what_they_replace(monkeypatch):
+    m = manager_with((4, 64))
+    be = m._be
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    be.entry("w").device = torch.device("cuda", 1)
+    assert be._import_device("w", None) == torch.device("cuda", 1)
+    assert be._import_device("w", "cuda:2") == torch.device("cuda", 2)
+    assert be._import_device("w", "cuda") == torch.device("cuda", 0)
+    assert be._import_device("w", "cpu") == torch.device("cuda", 1)       # stored bytes live on a GPU
+    assert be._import_device("new", None) == torch.device("cuda", 0)
+    assert be._import_device("new", torch.device("cpu")) == torch.device("cuda", 0)
+
+
+def test_a_converted_layer_is_loaded_where_it_is_asked_for(monkeypatch):
+    from neuzip_b200.mx4 import MX4Backend
+    went = []
+    monkeypatch.setattr(MX4Backend, "import_entry", lambda self, name, blob, device=None: went.append((name, device)))
+    m = neuzip.MX4Manager()
+    model = torch.nn.Sequential(torch.nn.Linear(64, 4, bias=False, device="meta"))
+    m.load_converted(model, {"0._extra_state": blob_of(), "0._p": torch.zeros(0)}, device="cpu")
+    assert went == [("0", "cpu")]
+    m.import_entry(blob_of(), "0")
+    assert went[1] == ("0", None)
