@@ -160,3 +160,11 @@ def test_a_converted_layer_is_loaded_where_it_is_asked_for(monkeypatch):
     assert went == [("0", "cpu")]
     m.import_entry(blob_of(), "0")
     assert went[1] == ("0", None)
+
+
+@pytest.mark.parametrize("dtype", ("bfloat16", "float16"))
+def test_a_loaded_layer_has_the_type_that_was_written(monkeypatch, dtype):
+    from neuzip_b200.mx4 import MX4Backend
+    monkeypatch.setattr(MX4Backend, "import_entry", lambda self, name, blob, device=None: None)
+    lin = neuzip.nn.Linear.from_compressed(neuzip.MX4Manager(), blob_of(dtype=dtype), device="cpu")
+    assert lin.weight.dtype == getattr(torch, dtype)
