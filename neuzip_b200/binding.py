@@ -72,6 +72,11 @@ class Manager:
             self._be = factory(algorithm.value, chunk_size)
         self.meta_dict: Dict[str, torch.Size] = {}
 
+    def _refused(self, handle: str, old: Optional[torch.Size]) -> None:
+        """What was to replace `handle` was not stored: its old shape still describes what it holds."""
+        if old is not None:
+            self.meta_dict[handle] = old
+
     def write(self, tensor: torch.Tensor, handle: Optional[str] = None,
               operand: Optional[bool] = None) -> str:
         """Compress ``tensor`` and return its handle; an existing handle is replaced.
@@ -80,11 +85,16 @@ class Manager:
         `read` returns is the same either way."""
         if handle is None:
             handle = str(len(self.meta_dict))
+        old = self.meta_dict.get(handle)
         self.meta_dict[handle] = tensor.shape
-        if operand is None or not getattr(self._be, "supports_operand_order", False):
-            self._be.write(handle, tensor)
-        else:
-            self._be.write(handle, tensor, operand=operand)
+        try:
+            if operand is None or not getattr(self._be, "supports_operand_order", False):
+                self._be.write(handle, tensor)
+            else:
+                self._be.write(handle, tensor, operand=operand)
+        except BaseException:
+            self._refused(handle, old)
+            raise
         return handle
 
     def read(self, handle: str) -> torch.Tensor:
@@ -211,8 +221,13 @@ class Manager:
         """Register compressed bytes produced by `export_entry` under a handle."""
         if handle is None:
             handle = str(len(self.meta_dict))
+        old = self.meta_dict.get(handle)
         self.meta_dict[handle] = torch.Size(blob["shape"])
-        self._be.import_entry(handle, blob)
+        try:
+            self._be.import_entry(handle, blob)
+        except BaseException:
+            self._refused(handle, old)
+            raise
         return handle
 
     def check(self) -> None:
@@ -253,8 +268,13 @@ class MX4Manager(Manager):
         holds `handle` already, else the current one)."""
         if handle is None:
             handle = str(len(self.meta_dict))
+        old = self.meta_dict.get(handle)
         self.meta_dict[handle] = torch.Size(blob["shape"])
-        self._be.import_entry(handle, blob, device)
+        try:
+            self._be.import_entry(handle, blob, device)
+        except BaseException:
+            self._refused(handle, old)
+            raise
         return handle
 
     def captured_bytes(self) -> int:
