@@ -128,6 +128,11 @@ class MX4Backend:
     def _status_of(self, device: int) -> torch.Tensor:
         word = self._status.get(device)
         if word is None:
+            if torch._C._cuda_isCurrentStreamCapturing():
+                # a word made here would be the graph's: without a value before the first replay, and cleared
+                # by every one
+                raise RuntimeError("a manager's first product or row lookup on a device cannot be captured in a "
+                                   "CUDA graph: make one before the capture")
             _lib.check(self._lib.nz_device_check())
             word = self._status[device] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
         return word
@@ -188,7 +193,7 @@ class MX4Backend:
         source = tensor if tensor.is_contiguous() else tensor.detach().contiguous()
         with _on(source.device):
             device = source.get_device()
-            if device not in self._status:
+            if device not in self._status and not torch._C._cuda_isCurrentStreamCapturing():
                 self._status_of(device)
             shape = source.shape
             matrices, rows, cols = _stack(shape)
@@ -350,7 +355,9 @@ class MX4Backend:
         workspace = x.new_empty(need, dtype=torch.uint8) if need else None
         if bias is not None:
             bias = bias.contiguous()
-        status = self._status[device]
+        status = self._status.get(device)
+        if status is None:
+            status = self._status_of(device)
         rc = self._lib.nz_mx4_linear(
             entry.packed.data_ptr(), entry.matrices, entry.rows, entry.cols, _DTYPES[x.dtype], x.data_ptr(),
             x.stride(0), n_rows, per_input, None if ids is None else ids.data_ptr(),
@@ -393,7 +400,8 @@ class MX4Backend:
         device = self._import_device(name, device)
         with _on(device):
             packed = blob["packed"].to(device=device, copy=True).contiguous()
-            self._status_of(device.index)
+            if not torch._C._cuda_isCurrentStreamCapturing():
+                self._status_of(device.index)
             self._cache[name] = _Entry(shape, dtype, *stack, packed,
                                        {torch._C._cuda_getCurrentRawStream(device.index)})
 

@@ -153,3 +153,30 @@ def test_a_checkpoint_is_loaded_onto_the_devices_of_its_layers():
         x = rand(341, 3, 64)
         mx4ref.check(m.linear("e", x.to("cuda:1")), *mx4ref.product(x, w))
     m.check()
+
+
+def test_the_first_call_of_a_manager_is_a_captured_one():
+    """A write is quantised at every replay; products and row lookups need the status word, which has to be
+    there before, so that no replay clears what other calls have reported."""
+    from neuzip_b200 import _lib
+    w, x = rand(350, 60, 96).cuda(), rand(351, 5, 96).cuda()
+    m = neuzip.MX4Manager()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h = m.write(w)
+        got = m.read(h)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            m.linear(h, x)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            m.read_rows(h, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    assert not m._be._status
+    graph.replay()
+    assert torch.equal(got.cpu().double(), mx4ref.quantize(w))
+    m.check()
+    m.read_rows(h, torch.tensor([60]).cuda())
+    w.neg_()
+    graph.replay()
+    assert torch.equal(got.cpu().double(), mx4ref.quantize(w))
+    with pytest.raises(_lib.NeuzipError, match="out of range"):
+        m.check()

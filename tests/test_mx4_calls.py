@@ -168,3 +168,12 @@ def test_a_loaded_layer_has_the_type_that_was_written(monkeypatch, dtype):
     monkeypatch.setattr(MX4Backend, "import_entry", lambda self, name, blob, device=None: None)
     lin = neuzip.nn.Linear.from_compressed(neuzip.MX4Manager(), blob_of(dtype=dtype), device="cpu")
     assert lin.weight.dtype == getattr(torch, dtype)
+
+
+def test_the_status_word_is_not_made_inside_a_capture(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True)
+    be = neuzip.MX4Manager()._be
+    with pytest.raises(RuntimeError, match="before the capture"):
+        be._status_of(0)
+    be._status[0] = word = torch.zeros(1, dtype=torch.int32)
+    assert be._status_of(0) is word
