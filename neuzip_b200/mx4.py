@@ -243,6 +243,7 @@ class MX4Backend:
             if row_len % entry.cols:
                 raise ValueError(f"row length {row_len} is not a whole number of stored rows")
             run = row_len // entry.cols
+            rows = rows.clamp(-1, entry.numel // row_len)     # far numbers times `run` could wrap into the table
             rows = (rows.unsqueeze(1) * run + torch.arange(run, device=device)).reshape(-1)
         with _on(device):
             out = torch.empty(rows.numel(), entry.cols, dtype=entry.dtype, device=device)

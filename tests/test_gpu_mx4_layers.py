@@ -180,3 +180,15 @@ def test_the_first_call_of_a_manager_is_a_captured_one():
     assert torch.equal(got.cpu().double(), mx4ref.quantize(w))
     with pytest.raises(_lib.NeuzipError, match="out of range"):
         m.check()
+
+
+@pytest.mark.parametrize("far", (20, -1, 2 ** 62, -2 ** 62, 2 ** 63 - 1, -2 ** 63))
+def test_rows_far_outside_a_table_of_several_dimensions(far):
+    from neuzip_b200 import _lib
+    m = neuzip.MX4Manager()
+    w = rand(360, 20, 4, 40)
+    h = m.write(w.cuda())
+    got = m.read_rows(h, torch.tensor([far, 19]).cuda()).cpu()
+    assert not got[0].any() and torch.equal(got[1].double(), mx4ref.quantize(w)[19])
+    with pytest.raises(_lib.NeuzipError, match="out of range"):
+        m.check()
