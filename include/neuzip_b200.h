@@ -509,6 +509,16 @@ int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t rows, uint64_t
                   const void *experts, const void *bias, void *y, void *workspace,
                   uint64_t workspace_bytes, void *status, void *stream);
 
+/* How nz_mx4_linear runs a product of these sizes on the current device: one of the NZ_MX4_*
+ * below, or -1 where there is nothing to run or the product is too large for one call.  For tests
+ * and logs; results do not depend on it but for the order of the sums. */
+#define NZ_MX4_FEW_ROWS 0      /* on the CUDA cores */
+#define NZ_MX4_ONE_LAUNCH 1    /* CTAs quantise the rows of x that they multiply */
+#define NZ_MX4_WHOLE_TILES 2   /* x is quantised by a kernel of its own */
+#define NZ_MX4_SHARED_TILES 3  /* the same, and CTAs share the steps of a tile */
+#define NZ_MX4_PAIRS 4         /* the same, whole tiles in pairs of CTAs */
+int nz_mx4_linear_way(uint64_t matrices, uint64_t rows, uint64_t cols, uint64_t n_rows, int grouped);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,11 +119,13 @@ SIGNATURES["nz_peer_close"] = (_int, [_vp])
 SIGNATURES["nz_peer_free"] = (_int, [_vp])
 
 NZ_DTYPE_BF16, NZ_DTYPE_FP16 = 0, 1
+(NZ_MX4_FEW_ROWS, NZ_MX4_ONE_LAUNCH, NZ_MX4_WHOLE_TILES, NZ_MX4_SHARED_TILES, NZ_MX4_PAIRS) = range(5)
 SIGNATURES["nz_mx4_bytes"] = (_u64, [_u64, _u64, _u64])
 SIGNATURES["nz_mx4_quantize"] = (_int, [_vp, _int, _u64, _u64, _u64, _vp, _vp])
 SIGNATURES["nz_mx4_dequantize"] = (_int, [_vp, _u64, _u64, _u64, _int, _vp, _vp])
 SIGNATURES["nz_mx4_gather_rows"] = (_int, [_vp, _u64, _u64, _u64, _int, _vp, _u64, _vp, _vp, _vp])
 SIGNATURES["nz_mx4_linear_workspace_bytes"] = (_u64, [_u64, _u64, _u64, _u64, _int])
+SIGNATURES["nz_mx4_linear_way"] = (_int, [_u64, _u64, _u64, _u64, _int])
 SIGNATURES["nz_mx4_linear"] = (
     _int, [_vp, _u64, _u64, _u64, _int, _vp, _u64, _u64, _u64, _vp, _vp, _vp, _vp, _u64, _vp, _vp])
 

@@ -1412,6 +1412,16 @@ extern "C" uint64_t nz_mx4_linear_workspace_bytes(uint64_t matrices, uint64_t ro
   return g.bytes;
 }
 
+extern "C" int nz_mx4_linear_way(uint64_t matrices, uint64_t rows, uint64_t cols, uint64_t n_rows, int grouped) {
+  using namespace nz;
+  const MxShape w{matrices, rows, cols};
+  MxPlan g;
+  if (matrices == 0 || rows == 0 || cols == 0 || n_rows == 0) return -1;
+  if (mx_few_rows(w, n_rows, grouped != 0)) return NZ_MX4_FEW_ROWS;
+  if (!mx_plan(w, n_rows, grouped != 0, g)) return -1;
+  return g.fused ? NZ_MX4_ONE_LAUNCH : g.pair ? NZ_MX4_PAIRS : g.split ? NZ_MX4_SHARED_TILES : NZ_MX4_WHOLE_TILES;
+}
+
 extern "C" int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t rows, uint64_t cols, int dtype,
                              const void *x, uint64_t x_stride, uint64_t n_rows, uint64_t per_input,
                              const void *experts, const void *bias, void *y, void *workspace,

@@ -177,3 +177,11 @@ def test_the_status_word_is_not_made_inside_a_capture(monkeypatch):
         be._status_of(0)
     be._status[0] = word = torch.zeros(1, dtype=torch.int32)
     assert be._status_of(0) is word
+
+
+def test_way_of_running_of_calls_with_nothing_to_run():
+    from neuzip_b200 import _lib
+    L = _lib.load()
+    for sizes in ((1, 0, 64, 4), (1, 64, 0, 4), (1, 64, 64, 0), (0, 64, 64, 4)):
+        assert L.nz_mx4_linear_way(*sizes, 0) == -1
+    assert L.nz_mx4_linear_way(1, 64, 64, 1, 0) == _lib.NZ_MX4_FEW_ROWS
