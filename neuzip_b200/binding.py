@@ -240,7 +240,8 @@ class Manager:
 
 
 class MX4Manager(Manager):
-    """A manager that holds tensors in microscaled 4-bit floating point (4.25 bits an element,
+    """A manager that holds tensors in microscaled 4-bit floating point (4.25 bits an element where
+    matrices have a multiple of 128 rows and 256 columns, more where they are filled up to that;
     lossy) instead of compressing them, and whose `linear` multiplies the stored form on the
     tensor cores, inputs quantised on the way (:mod:`neuzip_b200.mx4`).  Same methods as
     :class:`Manager`; bf16 and fp16 tensors; `read` returns the stored numbers in the type that

@@ -3,7 +3,11 @@ them as they are: the counterpart of :class:`neuzip_b200.backend.CodecBackend` w
 methods, over the ``nz_mx4_*`` calls of ``libneuzip_b200.so``.
 
 Every 32 consecutive elements of the last dimension share a power of two; an element keeps a
-sign, two exponent bits and one mantissa bit, 4.25 bits in all.  `linear` and
+sign, two exponent bits and one mantissa bit, 4.25 bits in all.  That holds for matrices with a multiple
+of 128 rows and of 256 columns: every matrix is stored in tiles of 128 rows, columns in blocks of 32
+with scales for 256 at a time, all filled up.  Low or narrow tensors take more (128 x 32 6 bits an
+element, matrices of 16 rows eight times their share, a vector of 4096 elements 544 bits an element);
+`size` counts it all.  `linear` and
 `grouped_linear` quantise their inputs by the same rule, so that the tensor cores multiply
 4-bit operands directly; the weights are never decoded.  The reference has no such form: its
 lossy precisions (cuda/kernels.cuh:53-156) keep entropy-coded exponents and decompress before
@@ -85,9 +89,7 @@ def _workspace_bytes(device: int, matrices: int, rows: int, cols: int, n_rows: i
 
 
 def _has_tangent(tensor: Optional[torch.Tensor]) -> bool:
-    # outside every dual_level there is nothing to unpack (which takes 0.4 us)
-    return (tensor is not None and getattr(forward_ad, "_current_level", 0) >= 0
-            and forward_ad.unpack_dual(tensor).tangent is not None)
+    return tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None
 
 
 def _in_autocast_type(tensor: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -269,15 +271,16 @@ class MX4Backend:
             raise ValueError(f"linear needs a matrix, got a tensor of shape {tuple(shape)}")
         if torch.is_autocast_enabled():
             input, bias = _in_autocast_type(input), _in_autocast_type(bias)
-        x = self._checked_input(entry, input, bias, (entry.rows,))
+        x = self._checked_input(entry, input, bias, False)
         if bias is not None and bias.requires_grad and torch.is_grad_enabled():
             return _TrainedBias.apply(bias, self._dense, entry, x, input)
         return self._dense(entry, x, input, bias)
 
     def _dense(self, entry: _Entry, x: torch.Tensor, input: torch.Tensor,
                bias: Optional[torch.Tensor]) -> torch.Tensor:
-        y = input.new_empty((*input.shape[:-1], entry.rows))
-        return self._launch(entry, x, x.shape[0], 1, None, bias, y)
+        n = x.size(0)
+        y = input.new_empty((n, entry.rows) if input.dim() == 2 else (*input.shape[:-1], entry.rows))
+        return self._launch(entry, x, n, 1, None, bias, y)
 
     def linear_without_bias(self, name: str, input: torch.Tensor, shape: Sequence[int]) -> torch.Tensor:
         return self.linear(name, input, shape)
@@ -306,7 +309,7 @@ class MX4Backend:
             per_input = int(experts.shape[-1])
         if torch.is_autocast_enabled():
             input, bias = _in_autocast_type(input), _in_autocast_type(bias)
-        x = self._checked_input(entry, input, bias, (entry.matrices, entry.rows))
+        x = self._checked_input(entry, input, bias, True)
         if bias is not None and bias.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("grouped_linear has no gradient for its bias: detach it, or call under "
                                "torch.no_grad()")
@@ -315,7 +318,7 @@ class MX4Backend:
         return self._launch(entry, x, ids.numel(), per_input, ids, bias, y)
 
     def _checked_input(self, entry: _Entry, input: torch.Tensor,
-                       bias: Optional[torch.Tensor], bias_shape) -> torch.Tensor:
+                       bias: Optional[torch.Tensor], stack: bool) -> torch.Tensor:
         """`input` as rows one element apart inside, after the checks the products share."""
         if input.dtype not in _DTYPES:
             raise RuntimeError("Unsupported data type")
@@ -330,12 +333,14 @@ class MX4Backend:
                 raise ValueError(f"bias must be of type {_NAMES[input.dtype]} on {entry.device}, got "
                                  f"{bias.dtype} on {bias.device}")
             # a vector's numbers have one order whatever its shape, those of a stack do not
-            if bias.shape != bias_shape and (len(bias_shape) > 1 or bias.numel() != entry.rows):
-                raise ValueError(f"bias must have the shape {bias_shape}, got {tuple(bias.shape)}")
+            if bias.shape != (entry.matrices, entry.rows) if stack else bias.numel() != entry.rows:
+                raise ValueError(f"bias must have the shape {(entry.matrices, entry.rows) if stack else (entry.rows,)}, "
+                                 f"got {tuple(bias.shape)}")
         if input.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("a manager's products with 4-bit weights have no gradient for their inputs: use "
                                "nn.Linear for one matrix, or call under torch.no_grad()")
-        if _has_tangent(input) or _has_tangent(bias):
+        # outside every dual_level there is nothing to unpack (which takes 0.4 us)
+        if getattr(forward_ad, "_current_level", 0) >= 0 and (_has_tangent(input) or _has_tangent(bias)):
             raise NotImplementedError("products with 4-bit weights have no forward-mode derivative")
         x = input if len(shape) == 2 else input.reshape(-1, entry.cols)
         row, element = x.stride()

@@ -185,3 +185,10 @@ def test_way_of_running_of_calls_with_nothing_to_run():
     for sizes in ((1, 0, 64, 4), (1, 64, 0, 4), (1, 64, 64, 0), (0, 64, 64, 4)):
         assert L.nz_mx4_linear_way(*sizes, 0) == -1
     assert L.nz_mx4_linear_way(1, 64, 64, 1, 0) == _lib.NZ_MX4_FEW_ROWS
+
+
+def test_bytes_of_tensors_that_fill_no_tile():
+    # what the module's text says: bits an element
+    for shape, bits in (((128, 256), 4.25), (((128, 32)), 6.0), ((4096,), 544.0), ((8, 16, 4096), 34.0)):
+        m = manager_with(shape)
+        assert m.size("w") * 8 / torch.Size(shape).numel() == bits
