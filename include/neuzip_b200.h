@@ -500,7 +500,7 @@ int nz_mx4_gather_rows(const void *packed, uint64_t matrices, uint64_t rows, uin
  * experts[r] = -1 gives a row of zeros; any other number outside 0 .. matrices - 1 too,
  * and sets NZ_STATUS_BAD_INDEX.  The workspace is 256-byte aligned, of
  * nz_mx4_linear_workspace_bytes bytes for the current device (`grouped`: with experts;
- * 0 for few rows), needs no set-up and is free again when the call's work is done.
+ * 0 where none is needed), needs no set-up and is free again when the call's work is done.
  * The results do not depend on the order in which blocks run. */
 uint64_t nz_mx4_linear_workspace_bytes(uint64_t matrices, uint64_t rows, uint64_t cols,
                                        uint64_t n_rows, int grouped);

@@ -212,8 +212,8 @@ __global__ void __launch_bounds__(kMxFewWarps * 32, 1) mx4_few_kernel(const MxFe
 
 // Whether a product goes this way: what the CUDA cores have to do, rows of y times elements of a
 // matrix, decides.  Measured against the tensor cores' way, in us: one row 4096 x 4096 (16.8 M) 5.6 : 8.2,
-// 8192 x 8192 13.8 : 12.8; 1024 x 1024 one row 4.7 : 5.9, two 5.5 : 5.8, four 7.9 : 5.8; one token to 8
-// experts 1408 x 2048 (23 M) 8.7 : 9.5.
+// 8192 x 8192 13.8 : 12.8; 1024 x 1024 one row 4.6 : 5.8, two 5.4 : 5.8, four 7.9 : 5.8; one token to 8
+// experts 1408 x 2048 (23 M) 8.5 : 8.9, where a step more of columns begins to turn it (1408 x 2080 9.3 : 8.9).
 bool mx_few_rows(const MxShape &w, uint64_t n_rows, bool grouped) {
   if ((grouped ? 1 : n_rows) * (w.blocks() * 65) > kMxFewSmem) return false;
   if (n_rows > (grouped ? kMxFewRows : 2)) return false;

@@ -17,7 +17,7 @@
 // Ways of running, chosen by an estimate of their times (mx_cost) from sizes alone:
 //   few     (nz_mx4_few.cu) one or two rows, or some rows of a stack, on the CUDA cores
 //   fused   one launch; every CTA quantises the rows of its slots itself, into shared memory, by 12 warps.
-//           The less host time (one launch, no workspace), and no longer up to about 4 rows of 4096
+//           The less host time (one launch, no workspace); up to about 4 rows it takes 1 us more on the device
 //   alone   a kernel quantises x into the workspace, and the product reads W meanwhile (a programmatic
 //           dependent launch): its ring is full of W when the inputs come
 //   shared  the same, and the steps of all tiles are divided evenly over the SMs, not tiles; the CTA that
@@ -25,14 +25,16 @@
 //           who is last
 //   pair    two CTAs with cta_group::2: 256 rows of W, half of a slot's step each.  A step then brings 34
 //           instead of 51 KB into an SM.  Large products are bound by that traffic and the power it
-//           takes: 8192 x 8192 x 28672 took 1293 us alone and takes 790 in pairs under sustained load, and
-//           580 if nothing but scales were copied
+//           takes: 8192 rows x 8192 x 28672 took 1293 us alone and takes 730 to 790 in pairs under sustained
+//           load, and 580 if nothing but scales were copied
 // Rows find their slots in every block (up to 1024 rows and 256 matrices) or by a kernel of one block.
 //
-// Measured on a B200, cold weights, in a graph (the bytes at 6.54 TB/s in brackets, in us): 16 rows x 4096
-// x 11008 9.5 (3.7), 8192 x 8192 13.2 (5.4), 8192 x 28672 26.0 (19.1); 64 experts 1408 x 2048, 32 tokens
-// to 8 each 23.3 (14.8).  What is over the bytes is a constant 6 to 7 us: two launches (2), the first
-// bytes' latency (2), the last step's products and stores (1), the end of the grid (1).
+// Measured on a B200, cold weights, in a graph (the bytes at 6.54 TB/s in brackets, in us; rows x inner x
+// outer size): 16 x 4096 x 11008 9.7 (3.7), 16 x 8192 x 8192 12.5 (5.4), 16 x 8192 x 28672 24.7 (19.1);
+// 64 experts 2048 x 1408, 32 tokens to 8 each 22.3 (14.8).  What is over the bytes is 6 to 7.5 us.  6 of them
+// are the same for all: two launches (2), the first bytes' latency (2), the last step's products and
+// stores (1), the end of the grid (1).  The rest grows with what is left uneven in the last wave of tiles
+// and, for experts, with finding the rows' slots in every block (1).
 #include <cuda.h>
 #include <math.h>
 #include <string.h>
@@ -1124,10 +1126,13 @@ struct MxPlan {
 // a cycle) and into all of them (7400 from L2; 3400 of W from memory).  A launch before the product costs
 // 5000 (its device time is hidden in part, its host time is not), a pair's start 2000 more, an item beside
 // its steps 300 and 8 a row.  The pieces of a shared tile are joined four at a time, 16 columns in 1800.
-// Against measurements, in us, this way and the next best: 16 rows x 4096 x 11008 alone 9.5, fused 14.0;
-// 4 rows fused 10.0, alone 9.6 and 4 more of host time; 4 rows x 8192 x 512 shared by a few CTAs a tile 9.4,
-// by 32 18.2, in whole tiles 11.9; 256 rows x 16384 x 2048 whole 21.9, shared 32.5; 4 rows x 16384 x 2048 shared 17.0,
-// whole 27.9; 2048 rows x 8192 x 28672 in pairs 190, alone 280; 64 rows x 4096 x 11008 alone 10.1, in pairs 11.1.
+// Measured in us on the device, what it chooses first (rows x inner x outer size, every way forced in turn):
+//   16 x 4096 x 11008 alone 9.7, pairs 10.7, fused 14.0, shared 14.2; 64 x 4096 x 11008 alone 10.2, pairs 11.1
+//   4 x 4096 x 11008 fused 10.7, alone 9.6 and 4 more of host time; 4 x 8192 x 512 shared 9.5, alone 11.5
+//   4 x 16384 x 2048 shared 12.2, alone 18.5; 16 x 16384 x 2048 shared 12.7, alone 18.5
+//   2048 x 4096 x 11008 pairs 45.4, alone 48.4; 2048 x 8192 x 28672 pairs 175, alone 223
+// Where it is off: 256 x 16384 x 2048 shared 23.8, alone 21.3; 256 x 2048 x 16384 pairs 14.2, alone 12.3;
+// 256 x 4096 x 11008 pairs 16.4, alone 15.8.
 enum MxKind { kMxWhole, kMxShared, kMxPaired, kMxOneLaunch };
 static double mx_cost(uint64_t tok, double slots, const MxShape &w, double n_rows, double hit, uint32_t sms,
                       MxKind kind, uint32_t &pieces) {
