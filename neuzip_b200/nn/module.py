@@ -27,16 +27,17 @@ class Parameter(torch.nn.Parameter):
         nothing is decompressed or compressed.  Not in the reference, which cannot load a
         converted model at all (its state_dict holds only the empty placeholder)."""
         device = device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu")
+        if getattr(manager, "keeps_devices", False):
+            handle = manager.import_entry(blob, device=device)
+        else:
+            handle = manager.import_entry(blob)
         # entries without a type are compressed bf16
         placeholder = torch.zeros(0, dtype=getattr(torch, blob.get("dtype", "bfloat16")), device=device)
         self = torch.nn.Parameter.__new__(cls, placeholder, True)
         self._manager = manager
         self._shape = torch.Size(blob["shape"])
         self._gradient = None
-        if getattr(manager, "keeps_devices", False):
-            self._handle = manager.import_entry(blob, device=device)
-        else:
-            self._handle = manager.import_entry(blob)
+        self._handle = handle
         self._staged = None
         self._stage_tag = None
         return self

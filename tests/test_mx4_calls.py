@@ -192,3 +192,9 @@ def test_bytes_of_tensors_that_fill_no_tile():
     for shape, bits in (((128, 256), 4.25), (((128, 32)), 6.0), ((4096,), 544.0), ((8, 16, 4096), 34.0)):
         m = manager_with(shape)
         assert m.size("w") * 8 / torch.Size(shape).numel() == bits
+
+
+@pytest.mark.parametrize("dtype", ("nonsense", "load", "float32"))
+def test_a_layer_of_an_unknown_type_is_refused_by_the_import(dtype):
+    with pytest.raises(ValueError, match="type"):
+        neuzip.nn.Linear.from_compressed(neuzip.MX4Manager(), blob_of(dtype="bfloat16") | {"dtype": dtype}, device="cpu")
