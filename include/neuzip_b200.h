@@ -510,7 +510,7 @@ int nz_mx4_linear(const void *packed, uint64_t matrices, uint64_t rows, uint64_t
                   uint64_t workspace_bytes, void *status, void *stream);
 
 /* How nz_mx4_linear runs a product of these sizes on the current device: one of the NZ_MX4_*
- * below, or -1 where there is nothing to run or the product is too large for one call.  For tests
+ * below, or -1 where there is nothing to run or the call would be refused for its sizes.  For tests
  * and logs; results do not depend on it but for the order of the sums. */
 #define NZ_MX4_FEW_ROWS 0      /* on the CUDA cores */
 #define NZ_MX4_ONE_LAUNCH 1    /* CTAs quantise the rows of x that they multiply */

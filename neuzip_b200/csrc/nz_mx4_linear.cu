@@ -1421,7 +1421,9 @@ extern "C" int nz_mx4_linear_way(uint64_t matrices, uint64_t rows, uint64_t cols
   using namespace nz;
   const MxShape w{matrices, rows, cols};
   MxPlan g;
-  if (matrices == 0 || rows == 0 || cols == 0 || n_rows == 0) return -1;
+  if (!mx_shape("nz_mx4_linear_way", matrices, rows, cols) || matrices == 0 || rows == 0 || cols == 0 ||
+      n_rows == 0 || n_rows >= (1ull << 31) || matrices > (grouped ? kMxMaxExperts : 1))
+    return -1;
   if (mx_few_rows(w, n_rows, grouped != 0)) return NZ_MX4_FEW_ROWS;
   if (!mx_plan(w, n_rows, grouped != 0, g)) return -1;
   return g.fused ? NZ_MX4_ONE_LAUNCH : g.pair ? NZ_MX4_PAIRS : g.split ? NZ_MX4_SHARED_TILES : NZ_MX4_WHOLE_TILES;

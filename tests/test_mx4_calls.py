@@ -198,3 +198,12 @@ def test_bytes_of_tensors_that_fill_no_tile():
 def test_a_layer_of_an_unknown_type_is_refused_by_the_import(dtype):
     with pytest.raises(ValueError, match="type"):
         neuzip.nn.Linear.from_compressed(neuzip.MX4Manager(), blob_of(dtype="bfloat16") | {"dtype": dtype}, device="cpu")
+
+
+def test_way_of_running_of_sizes_that_the_product_refuses():
+    from neuzip_b200 import _lib
+    way = _lib.load().nz_mx4_linear_way
+    for sizes in ((1, 1 << 31, 64, 4, 0), (1, 64, 1 << 31, 4, 0), (1, 64, 64, 1 << 31, 0), (2, 64, 64, 4, 0),
+                  (8193, 64, 64, 4, 1), (1 << 40, 1 << 40, 1 << 40, 1 << 40, 1), (1, 64, 64, (1 << 64) - 1, 0)):
+        assert way(*sizes) == -1, sizes
+    assert way(8192, 64, 64, 4, 1) == _lib.NZ_MX4_FEW_ROWS
