@@ -207,3 +207,13 @@ def test_way_of_running_of_sizes_that_the_product_refuses():
                   (8193, 64, 64, 4, 1), (1 << 40, 1 << 40, 1 << 40, 1 << 40, 1), (1, 64, 64, (1 << 64) - 1, 0)):
         assert way(*sizes) == -1, sizes
     assert way(8192, 64, 64, 4, 1) == _lib.NZ_MX4_FEW_ROWS
+
+
+def test_captured_bytes_are_not_released_inside_a_capture(monkeypatch):
+    m = manager_with((128, 32))
+    entry = m._be.entry("w")
+    m._be._captured[entry.packed.data_ptr()] = entry.packed
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True)
+    with pytest.raises(RuntimeError, match="inside the capture"):
+        m.release_captured()
+    assert len(m._be._captured) == 1
