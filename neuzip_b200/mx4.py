@@ -181,7 +181,7 @@ class MX4Backend:
         """Keep nothing more for the graphs that have been captured so far: those that read a handle
         must not be replayed after it is written again or erased.  Waits for the work under way, so
         not inside a capture."""
-        if self._captured and torch._C._cuda_isCurrentStreamCapturing():
+        if torch.cuda.is_initialized() and torch._C._cuda_isCurrentStreamCapturing():
             raise RuntimeError("release_captured cannot be called inside the capture of a CUDA graph")
         for device in {packed.device for packed in self._captured.values() if packed.is_cuda}:
             torch.cuda.synchronize(device)

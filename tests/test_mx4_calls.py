@@ -213,6 +213,7 @@ def test_captured_bytes_are_not_released_inside_a_capture(monkeypatch):
     m = manager_with((128, 32))
     entry = m._be.entry("w")
     m._be._captured[entry.packed.data_ptr()] = entry.packed
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
     monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True)
     with pytest.raises(RuntimeError, match="inside the capture"):
         m.release_captured()
