@@ -136,7 +136,10 @@ class MX4Backend:
                 raise RuntimeError("a manager's first product or row lookup on a device cannot be captured in a "
                                    "CUDA graph: make one before the capture")
             _lib.check(self._lib.nz_device_check())
-            word = self._status[device] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+            word = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+            # cleared before any stream may set it; where two threads come first together, one word stays
+            torch.cuda.current_stream(device).synchronize()
+            word = self._status.setdefault(device, word)
         return word
 
     def status(self) -> int:

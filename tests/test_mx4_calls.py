@@ -218,3 +218,22 @@ def test_captured_bytes_are_not_released_inside_a_capture(monkeypatch):
     with pytest.raises(RuntimeError, match="inside the capture"):
         m.release_captured()
     assert len(m._be._captured) == 1
+
+
+def test_threads_that_come_first_together_share_one_status_word(monkeypatch):
+    be = neuzip.MX4Manager()._be
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False)
+    monkeypatch.setattr(be, "_lib", type("L", (), {"nz_device_check": lambda self: 0})())
+    order = []
+    monkeypatch.setattr(torch.cuda, "current_stream",
+                        lambda device: type("S", (), {"synchronize": lambda self: order.append("cleared")})())
+    zeros = torch.zeros
+
+    def made(*shape, dtype, device):
+        monkeypatch.setattr(torch, "zeros", lambda *s, dtype, device: zeros(*s, dtype=dtype))
+        other.append(be._status_of(0))                       # the other thread, meanwhile
+        assert order == ["cleared"]
+        return zeros(*shape, dtype=dtype)
+    other = []
+    monkeypatch.setattr(torch, "zeros", made)
+    assert be._status_of(0) is other[0] is be._status[0] and order == ["cleared"] * 2
